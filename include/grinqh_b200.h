@@ -262,6 +262,81 @@ int grinqh_gemv_allreduce(const void *x_dev, int dtype, int64_t K, const uint32_
                           size_t workspace_bytes, int rank, int world, void *const *buffers_dev, int64_t cap,
                           int mode, grinqh_stream_t stream);
 
+/* ---------------------------------------------------------------------------------
+ * The attention block next to the linears: a paged KV cache held in 4 bits and the
+ * attention over prompts. (No reference counterparts: the reference leaves attention
+ * and its cache to vLLM.)
+ *
+ * cache_dev: uint8 [num_pages, num_kv_heads, page_size / 16, record], page_size a
+ * multiple of 16, 16-byte aligned. A record holds 16 consecutive tokens of one head in
+ * grinqh_kv4_record_bytes(head_dim, group_size) = 16 D + 128 NG bytes, D = head_dim,
+ * NG = D / group_size:
+ *   K codes   16 rows (tokens) of D/2 bytes; 32-bit word c*(D/32) + g*(group/32) + j of a
+ *             row holds channels g*group + c*group/4 + 8j + e at bits 4e (c 0..3, e 0..7)
+ *   V codes   8 rows (token pairs) of D bytes; word (c ^ 2(r%4))*(D/32) + g*(group/32) + j
+ *             of row r holds channels g*group + c*group/8 + 4j + e (c 0..7, e 0..3), of
+ *             token 2r at bits 4e, of token 2r+1 at bits 16+4e
+ *   K params  [16 tokens][NG] {scale, zero} in dtype; V params the same.
+ * A channel's value is scale * code + zero. head_dim 64 or 128; group_size 32, 64 or 128,
+ * at most head_dim.
+ * --------------------------------------------------------------------------------- */
+
+/* Bytes of a record; 0 for a head_dim or group_size that is not supported. */
+int64_t grinqh_kv4_record_bytes(int head_dim, int group_size);
+
+/* Quantize k, v [tokens, num_kv_heads, D] (strides in elements, D contiguous) into the
+ * cache; token i goes to place slots[i] = page * page_size + offset. Per token, head and
+ * group: zero = min x, scale = dtype((max - min) / 15), code = clamp(rint((x - zero) *
+ * (1 / scale)), 0, 15) in fp32 (0 for a scale below 2^-126). A slot outside the cache (-1 for
+ * padding) writes nothing; slots of one call must differ. k, v and their strides are
+ * 16-byte aligned. */
+int grinqh_kv4_append(const void *k, const void *v, int dtype, int64_t tokens, int num_kv_heads, int head_dim,
+                      int group_size, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                      int64_t v_head_stride, const int64_t *slots, uint8_t *cache, int64_t num_pages, int page_size,
+                      grinqh_stream_t stream);
+
+/* The values that the cache holds at slots[0..tokens): k, v [tokens, num_kv_heads, D]
+ * contiguous, 16-byte aligned, dtype(scale * code + zero). A slot outside the cache
+ * gives zeros. */
+int grinqh_kv4_gather(const uint8_t *cache, int dtype, int64_t num_pages, int page_size, int num_kv_heads,
+                      int head_dim, int group_size, const int64_t *slots, int64_t tokens, void *k, void *v,
+                      grinqh_stream_t stream);
+
+/* Attention of the last new_tokens tokens of every sequence over the cache:
+ *   query j of sequence b is token p = seq_lens[b] - new_tokens + j and sees tokens 0..p;
+ *   s_t = softmax_scale * q . k_t, out = sum_t softmax(s)_t v_t, lse = log sum_t exp(s_t);
+ *   a query that sees no token (p < 0) gives out = 0, lse = -inf.
+ * q [num_seqs, new_tokens, num_heads, D] (strides in elements, D contiguous, 16-byte
+ * aligned); token t of sequence b is in page block_tables[b * table_stride + t / page_size].
+ * seq_lens counts the new tokens; it is cut to table_width * page_size, and the tokens of
+ * a page outside the cache are left out. out [num_seqs, new_tokens, num_heads, D] dtype
+ * and lse [num_seqs, new_tokens, num_heads] fp32 are contiguous. num_heads is a multiple
+ * of num_kv_heads, new_tokens * num_heads / num_kv_heads at most 32.
+ * flags: GRINQH_WORKSPACE_ZEROED as for the linears. */
+size_t grinqh_kv4_attention_workspace_size(int64_t num_seqs, int new_tokens, int num_heads, int num_kv_heads,
+                                           int head_dim);
+int grinqh_kv4_attention(const void *q, int dtype, int64_t num_seqs, int new_tokens, int num_heads, int num_kv_heads,
+                         int head_dim, int group_size, int64_t q_seq_stride, int64_t q_token_stride,
+                         int64_t q_head_stride, const uint8_t *cache, int64_t num_pages, int page_size,
+                         const int32_t *block_tables, int64_t table_stride, int64_t table_width,
+                         const int32_t *seq_lens, float softmax_scale, void *out, float *lse, void *workspace,
+                         size_t workspace_bytes, int flags, grinqh_stream_t stream);
+
+/* Causal attention over packed sequences. Sequence b has the query rows
+ * cu_seqlens_q[b] .. cu_seqlens_q[b+1] of q [total_q, num_heads, D] and the key rows
+ * cu_seqlens_k[b] .. cu_seqlens_k[b+1] of k, v [total_k, num_kv_heads, D]; its n queries
+ * are the last of its m tokens: query j sees keys 0 .. m - n + j. Formulas, out and lse as
+ * for grinqh_kv4_attention; out [total_q, num_heads, D] and lse [total_q, num_heads] are
+ * contiguous, and rows that no sequence holds are not written. Strides in elements, D
+ * contiguous; pointers and strides 16-byte aligned. A key or value that is not finite may
+ * reach earlier queries of its own sequence (0 * inf is NaN), never another sequence. */
+int grinqh_prompt_attention(const void *q, const void *k, const void *v, int dtype, int64_t total_q, int64_t total_k,
+                            int num_seqs, int num_heads, int num_kv_heads, int head_dim, int64_t q_token_stride,
+                            int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                            int64_t v_token_stride, int64_t v_head_stride, const int32_t *cu_seqlens_q,
+                            const int32_t *cu_seqlens_k, float softmax_scale, void *out, float *lse,
+                            grinqh_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -437,6 +437,154 @@ std::tuple<at::Tensor, at::Tensor> grade(const at::Tensor& x, at::ArrayRef<doubl
   return {masks.view(shape), uni};
 }
 
+// ---------------------------------------------------------------- attention block
+// A tensor the C ABI can address: D contiguous, 16-byte aligned pointer and strides
+// (a view of a fused projection as it is); anything else is copied.
+at::Tensor rows16(const at::Tensor& t) {
+  bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && t.stride(i) % 8 == 0 && t.stride(i) >= 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+struct CacheShape {
+  int64_t pages, kv_heads, dim;
+  int page_size;
+};
+
+CacheShape check_cache(const at::Tensor& cache, int64_t group_size) {
+  check_cuda(cache, "cache");
+  TORCH_CHECK(cache.scalar_type() == at::kByte && cache.dim() == 4 && cache.is_contiguous(),
+              "GRINQH: cache must be a contiguous uint8 tensor [pages, kv heads, page_size / 16, record]");
+  TORCH_CHECK(group_size == 32 || group_size == 64 || group_size == 128,
+              "GRINQH: group_size must be 32, 64 or 128, got ", group_size);
+  const int64_t dim = cache.size(3) * group_size / (16 * group_size + 128);
+  TORCH_CHECK(grinqh_kv4_record_bytes((int)dim, (int)group_size) == cache.size(3) && cache.size(3) > 0,
+              "GRINQH: no head_dim has records of ", cache.size(3), " bytes with group_size ", group_size);
+  TORCH_CHECK(cache.size(2) > 0 && cache.size(2) < (int64_t(1) << 26), "GRINQH: cache has pages of ", cache.size(2),
+              " records");
+  return {cache.size(0), cache.size(1), dim, (int)(cache.size(2) * 16)};
+}
+
+void check_index(const at::Tensor& t, const char* name, at::ScalarType type, int64_t dim, const at::Tensor& like) {
+  TORCH_CHECK(t.device() == like.device(), "GRINQH: ", name, " is on ", t.device(), ", expected ", like.device());
+  TORCH_CHECK(t.scalar_type() == type && t.dim() == dim, "GRINQH: ", name, " must be a ", dim, "-D tensor of ", type);
+}
+
+void kv4_append(const at::Tensor& k, const at::Tensor& v, at::Tensor cache, const at::Tensor& slots,
+                int64_t group_size) {
+  const NvtxRange range("grinqh::kv4_append");
+  check_cuda(k, "k");
+  const int dt = dtype_code(k, "k");
+  const CacheShape c = check_cache(cache, group_size);
+  TORCH_CHECK(k.device() == cache.device() && v.device() == cache.device(), "GRINQH: k, v and cache must be on one GPU");
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(),
+              "GRINQH: k and v must be [tokens, kv heads, head_dim] of one type, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(k.size(1) == c.kv_heads && k.size(2) == c.dim, "GRINQH: k is ", k.sizes(), " but the cache holds ",
+              c.kv_heads, " heads of ", c.dim);
+  check_index(slots, "slots", at::kLong, 1, cache);
+  TORCH_CHECK(slots.size(0) == k.size(0), "GRINQH: one slot per token: ", slots.size(0), " for ", k.size(0), " tokens");
+  if (k.size(0) == 0) return;
+  const c10::cuda::CUDAGuard guard(k.device());
+  const at::Tensor kc = rows16(k), vc = rows16(v), sc = slots.contiguous();
+  check_ok(grinqh_kv4_append(kc.data_ptr(), vc.data_ptr(), dt, k.size(0), (int)c.kv_heads, (int)c.dim, (int)group_size,
+                             kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1), sc.data_ptr<int64_t>(),
+                             cache.data_ptr<uint8_t>(), c.pages, c.page_size, cur_stream(k)),
+           "kv4_append");
+}
+
+std::tuple<at::Tensor, at::Tensor> kv4_gather(const at::Tensor& cache, const at::Tensor& slots, int64_t group_size,
+                                              at::ScalarType dtype) {
+  const NvtxRange range("grinqh::kv4_gather");
+  const CacheShape c = check_cache(cache, group_size);
+  TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "GRINQH: dtype must be float16 or bfloat16, got ", dtype);
+  check_index(slots, "slots", at::kLong, 1, cache);
+  const c10::cuda::CUDAGuard guard(cache.device());
+  const at::Tensor sc = slots.contiguous();
+  at::Tensor k = at::empty({slots.size(0), c.kv_heads, c.dim}, cache.options().dtype(dtype));
+  at::Tensor v = at::empty_like(k);
+  if (k.numel())
+    check_ok(grinqh_kv4_gather(cache.data_ptr<uint8_t>(), dtype_code(k, "dtype"), c.pages, c.page_size, (int)c.kv_heads,
+                               (int)c.dim, (int)group_size, sc.data_ptr<int64_t>(), slots.size(0), k.data_ptr(),
+                               v.data_ptr(), cur_stream(cache)),
+             "kv4_gather");
+  return {k, v};
+}
+
+std::tuple<at::Tensor, at::Tensor> kv4_attention(const at::Tensor& q, const at::Tensor& cache,
+                                                 const at::Tensor& block_tables, const at::Tensor& seq_lens,
+                                                 int64_t group_size, double softmax_scale) {
+  const NvtxRange range("grinqh::kv4_attention");
+  check_cuda(q, "q");
+  const int dt = dtype_code(q, "q");
+  const CacheShape c = check_cache(cache, group_size);
+  TORCH_CHECK(q.device() == cache.device(), "GRINQH: q and cache must be on one GPU");
+  TORCH_CHECK(q.dim() == 3 || q.dim() == 4, "GRINQH: q must be [seqs, heads, head_dim] or [seqs, new tokens, heads, "
+              "head_dim], got ", q.sizes());
+  const int64_t seqs = q.size(0), fresh = q.dim() == 4 ? q.size(1) : 1, heads = q.size(-2);
+  TORCH_CHECK(q.size(-1) == c.dim, "GRINQH: q has head_dim ", q.size(-1), " but the cache ", c.dim);
+  TORCH_CHECK(heads > 0 && fresh > 0 && heads % c.kv_heads == 0, "GRINQH: ", heads,
+              " query heads are not a multiple of ", c.kv_heads, " kv heads (or there is no token)");
+  check_index(block_tables, "block_tables", at::kInt, 2, q);
+  check_index(seq_lens, "seq_lens", at::kInt, 1, q);
+  TORCH_CHECK(block_tables.size(0) == seqs && seq_lens.size(0) == seqs, "GRINQH: block_tables and seq_lens must have ",
+              seqs, " rows, got ", block_tables.size(0), " and ", seq_lens.size(0));
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor qc = rows16(q), lens = seq_lens.contiguous();
+  const at::Tensor tables = block_tables.stride(1) == 1 ? block_tables : block_tables.contiguous();
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor lse = at::empty(q.sizes().slice(0, q.dim() - 1), q.options().dtype(at::kFloat));
+  if (seqs == 0) return {out, lse};
+  const cudaStream_t stream = cur_stream(q);
+  const size_t bytes =
+      grinqh_kv4_attention_workspace_size(seqs, (int)fresh, (int)heads, (int)c.kv_heads, (int)c.dim);
+  at::Tensor ws;
+  bool zeroed = false;
+  if (bytes) ws = stream_workspace(q, bytes, stream, &zeroed);
+  check_ok(grinqh_kv4_attention(qc.data_ptr(), dt, seqs, (int)fresh, (int)heads, (int)c.kv_heads, (int)c.dim,
+                                (int)group_size, qc.stride(0), q.dim() == 4 ? qc.stride(1) : 0, qc.stride(-2),
+                                cache.data_ptr<uint8_t>(), c.pages, c.page_size, tables.data_ptr<int32_t>(),
+                                tables.stride(0), tables.size(1), lens.data_ptr<int32_t>(), (float)softmax_scale,
+                                out.data_ptr(), lse.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr,
+                                bytes ? static_cast<size_t>(ws.numel()) : 0, zeroed ? GRINQH_WORKSPACE_ZEROED : 0,
+                                stream),
+           "kv4_attention");
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor> prompt_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& cu_seqlens_q, const at::Tensor& cu_seqlens_k,
+                                                    double softmax_scale) {
+  const NvtxRange range("grinqh::prompt_attention");
+  check_cuda(q, "q");
+  const int dt = dtype_code(q, "q");
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device(), "GRINQH: q, k and v must be on one GPU");
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && k.size(2) == q.size(2),
+              "GRINQH: q must be [tokens, heads, head_dim], k and v [tokens, kv heads, head_dim], got ", q.sizes(),
+              ", ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+              "GRINQH: q, k and v must have one type");
+  TORCH_CHECK(k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0, "GRINQH: ", q.size(1),
+              " query heads are not a multiple of ", k.size(1), " kv heads");
+  check_index(cu_seqlens_q, "cu_seqlens_q", at::kInt, 1, q);
+  check_index(cu_seqlens_k, "cu_seqlens_k", at::kInt, 1, q);
+  TORCH_CHECK(cu_seqlens_q.size(0) >= 1 && cu_seqlens_q.size(0) == cu_seqlens_k.size(0),
+              "GRINQH: cu_seqlens_q and cu_seqlens_k must both have one entry more than there are sequences, got ",
+              cu_seqlens_q.size(0), " and ", cu_seqlens_k.size(0));
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor qc = rows16(q), kc = rows16(k), vc = rows16(v);
+  const at::Tensor cq = cu_seqlens_q.contiguous(), ck = cu_seqlens_k.contiguous();
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  if (out.numel() == 0) return {out, lse};
+  check_ok(grinqh_prompt_attention(qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), dt, q.size(0), k.size(0),
+                                   (int)(cq.size(0) - 1), (int)q.size(1), (int)k.size(1), (int)q.size(2), qc.stride(0),
+                                   qc.stride(1), kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1),
+                                   cq.data_ptr<int32_t>(), ck.data_ptr<int32_t>(), (float)softmax_scale,
+                                   out.data_ptr(), lse.data_ptr<float>(), cur_stream(q)),
+           "prompt_attention");
+  return {out, lse};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(grinqh, m) {
@@ -459,6 +607,12 @@ TORCH_LIBRARY(grinqh, m) {
   m.def("silu_mul_grade(Tensor x, float[] thresholds, int max_bits) -> (Tensor, Tensor, Tensor)");
   m.def("union_linear_masked(Tensor x, Tensor weight_packed, Tensor weight_scale, Tensor? bias, int max_bits, "
         "int group_size, int original_n, float[] thresholds, Tensor union_mask) -> Tensor");
+  m.def("kv4_append(Tensor k, Tensor v, Tensor(a!) cache, Tensor slots, int group_size) -> ()");
+  m.def("kv4_gather(Tensor cache, Tensor slots, int group_size, ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("kv4_attention(Tensor q, Tensor cache, Tensor block_tables, Tensor seq_lens, int group_size, "
+        "float softmax_scale) -> (Tensor, Tensor)");
+  m.def("prompt_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, "
+        "float softmax_scale) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(grinqh, CUDA, m) {
@@ -474,4 +628,8 @@ TORCH_LIBRARY_IMPL(grinqh, CUDA, m) {
   m.impl("rmsnorm_grade", &rmsnorm_grade);
   m.impl("silu_mul_grade", &silu_mul_grade);
   m.impl("union_linear_masked", &union_linear_masked);
+  m.impl("kv4_append", &kv4_append);
+  m.impl("kv4_gather", &kv4_gather);
+  m.impl("kv4_attention", &kv4_attention);
+  m.impl("prompt_attention", &prompt_attention);
 }

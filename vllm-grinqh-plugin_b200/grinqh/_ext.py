@@ -56,6 +56,15 @@ SIGNATURES = {
     "grinqh_rmsnorm_grade": (_int, [_ptr, _ptr, _ptr, _int, _i64, _i64, ctypes.c_float, _fptr, _int, _ptr, _ptr,
                                     _ptr, _ptr]),
     "grinqh_silu_mul_grade": (_int, [_ptr, _int, _i64, _i64, _fptr, _int, _ptr, _ptr, _ptr, _ptr]),
+    "grinqh_kv4_record_bytes": (_i64, [_int, _int]),
+    "grinqh_kv4_append": (_int, [_ptr, _ptr, _int, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _ptr, _ptr, _i64,
+                                 _int, _ptr]),
+    "grinqh_kv4_gather": (_int, [_ptr, _int, _i64, _int, _int, _int, _int, _ptr, _i64, _ptr, _ptr, _ptr]),
+    "grinqh_kv4_attention_workspace_size": (_size, [_i64, _int, _int, _int, _int]),
+    "grinqh_kv4_attention": (_int, [_ptr, _int, _i64, _int, _int, _int, _int, _int, _i64, _i64, _i64, _ptr, _i64, _int,
+                                    _ptr, _i64, _i64, _ptr, ctypes.c_float, _ptr, _ptr, _ptr, _size, _int, _ptr]),
+    "grinqh_prompt_attention": (_int, [_ptr, _ptr, _ptr, _int, _i64, _i64, _int, _int, _int, _int, _i64, _i64, _i64,
+                                       _i64, _i64, _i64, _ptr, _ptr, ctypes.c_float, _ptr, _ptr, _ptr]),
     "grinqh_gemv_noalloc": (_int, [_ptr, _int, _i64, _ptr, _ptr, _ptr, _int, _int, _i64, _fptr, _ptr, _ptr]),
 }
 
