@@ -305,7 +305,7 @@ int grinqh_kv4_gather(const uint8_t *cache, int dtype, int64_t num_pages, int pa
 /* Attention of the last new_tokens tokens of every sequence over the cache:
  *   query j of sequence b is token p = seq_lens[b] - new_tokens + j and sees tokens 0..p;
  *   s_t = softmax_scale * q . k_t, out = sum_t softmax(s)_t v_t, lse = log sum_t exp(s_t);
- *   a query that sees no token (p < 0) gives out = 0, lse = -inf.
+ *   a query that sees no token (p < 0) gives out = 0, lse = -inf. softmax_scale > 0.
  * q [num_seqs, new_tokens, num_heads, D] (strides in elements, D contiguous, 16-byte
  * aligned); token t of sequence b is in page block_tables[b * table_stride + t / page_size].
  * seq_lens counts the new tokens; it is cut to table_width * page_size, and the tokens of

@@ -406,6 +406,10 @@ def test_refusals():
         lambda: G.grinqh_kv4_attention(q, cache, tables, lens.long()),
         lambda: G.grinqh_kv4_attention(q, cache, tables, lens.repeat(2)),
         lambda: G.grinqh_kv4_attention(q.expand(1, 9, 8, 128), cache, tables, lens),
+        lambda: G.grinqh_kv4_attention(q, cache, tables, lens, 128, -1.0),
+        lambda: G.grinqh_kv4_attention(q, cache, tables, lens, 128, math.nan),
+        lambda: G.grinqh_prompt_attention(k, k, k, cu, cu, 0.0),
+        lambda: G.grinqh_prompt_attention(k, k, k, cu, cu, math.inf),
         lambda: G.grinqh_prompt_attention(k, k.half(), k.half(), cu, cu),
         lambda: G.grinqh_prompt_attention(k[:, :1], k, k, cu, cu),
         lambda: G.grinqh_prompt_attention(k, k, k[:2], cu, cu),

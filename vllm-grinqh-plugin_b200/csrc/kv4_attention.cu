@@ -101,6 +101,7 @@ extern "C" int grinqh_kv4_attention(const void* q, int dtype, int64_t num_seqs, 
   GRINQH_REQUIRE(num_seqs >= 0 && num_seqs <= 65535, "num_seqs out of range (%lld)", (long long)num_seqs);
   GRINQH_REQUIRE(table_width >= 0 && table_width * page_size < (1LL << 31) && (num_seqs <= 1 || table_stride >= 0),
                  "block_tables out of range");
+  GRINQH_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "softmax_scale must be positive and finite");
   if (num_seqs == 0) return GRINQH_OK;
   GRINQH_REQUIRE(q && seq_lens && out && lse && (block_tables || table_width == 0), "null pointer");
   GRINQH_REQUIRE(aligned(q, 16) && q_seq_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 &&
