@@ -12,6 +12,7 @@
 #include "decode_tc.cuh"
 #include "gemm_skinny.cuh"
 #include "gemm_bf16.cuh"
+#include "kv4_attention.cuh"
 #include "prompt_attention.cuh"
 
 namespace grinqh {
@@ -641,7 +642,7 @@ extern "C" int grinqh_gemv_allreduce(const void* x, int dtype, int64_t K, const 
 extern "C" int grinqh_take_error_flags(unsigned* timeouts) {
   GRINQH_RETURN_IF(check_device());
   const unsigned v = take_gemm_timeouts() + take_m1tc_timeouts() + take_skinny_timeouts() + take_bf16_gemm_timeouts() +
-                     take_m1_timeouts() + take_prompt_timeouts();
+                     take_m1_timeouts() + take_prompt_timeouts() + take_kv4_timeouts();
   if (timeouts) *timeouts = v;
   return GRINQH_OK;
 }
