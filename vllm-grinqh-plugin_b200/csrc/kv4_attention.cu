@@ -29,13 +29,14 @@
 #include "ptx.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace grinqh {
 namespace {
 
 constexpr int kMaxRows = 32;  // new tokens x query heads of a kv head
 constexpr float kSlack = 8.0f;       // weights may reach 2^kSlack before the running maximum follows
-constexpr float kTopWeight = 64.0f;  // weights x V scales stay below this x 2^kSlack, in f16's range
+constexpr float kTopWeight = 64.0f;  // V scales x vf stay below this, weights x that in f16's range
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr uint32_t kFull = 0xffffffffu;
 
@@ -61,12 +62,14 @@ struct Kv4AttnArgs {
 template <int D, int GS, int NT>
 struct Plan {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kWarps = NT == 1 ? 8 : 4;
+  // 8 warps, or as many as keep two CTAs on an SM
+  static constexpr int kWarps = NT == 2 ? 4 : (D == 128 && GS == 32 ? 6 : 8);
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kStages = D == 64 ? 6 : (Kv4<D, GS>::NG == 4 && NT == 1 ? 3 : 4);
+  static constexpr int kStages = D == 64 ? 3 : 2;        // of two records each
+  static constexpr uint32_t kStage = 2 * Kv4<D, GS>::kRecord;
   static constexpr int kRow = D + 4;                     // floats of a row of sums in shared memory
   static constexpr int kSums = kRows * kRow + 2 * kRows;  // O, m, l
-  static constexpr uint32_t kWarpRing = kStages * Kv4<D, GS>::kRecord;
+  static constexpr uint32_t kWarpRing = kStages * kStage;
   static constexpr uint32_t kSmem = kWarps * (kWarpRing + kSums * 4 + kStages * 8) + 512;
   // as many as 228 KB of shared memory and the registers let an SM hold
   static constexpr int kCtas = NT == 2 && 3 * (kSmem + 1024) <= 233472 ? 3 : 2;
@@ -248,18 +251,25 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
   if (x < end) advance(a, seg, warp * per, same);
 
   // ---------------------------------------------------------------- the warp's loads
-  // The record at `ld` is next to be loaded, into ring stage `put`. Page numbers are read
-  // a record or a page before they are needed.
-  int ld_x = x, put = 0;
+  // A stage takes the next two records of a sequence and head (the last of them alone may
+  // be one): one copy where they lie in one page. Page numbers are read a page ahead.
+  int ld_x = x, put = 0;  // place of the next record to load; stage it goes to
   Pos ld = seg;
   int page = 0, page_next = 0, in_page = 0, entry = 0;
-  uint32_t skipped = 0;  // bit per stage: page outside the cache, nothing was loaded
-  auto enter = [&] {     // a sequence and head
+  const uint8_t* src = nullptr;
+  uint32_t bad = 0;  // two bits per stage: record of a page outside the cache, not loaded
+  auto find = [&] {  // the record at in_page of `page`
+    src = page >= 0 && page < a.pages
+              ? a.cache + (((int64_t)page * a.kv_heads + ld.h / a.parts) * a.page_tiles + in_page) * L::kRecord
+              : nullptr;
+  };
+  auto enter = [&] {  // a sequence and head
     entry = ld.at / a.page_tiles;
     in_page = ld.at - entry * a.page_tiles;
     const int32_t* table = a.tables + ld.b * a.table_stride;
     page = table[entry];
     page_next = table[min(entry + 1, (ld.nt - 1) / a.page_tiles)];
+    find();
   };
   auto settle = [&] {  // from a place that is no record to the next one that is
     while (ld_x < end && ld.at >= ld.nt) {
@@ -271,31 +281,53 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
       }
     }
   };
-  auto load = [&] {
-    if (ld_x >= end) return;
-    const bool ok = page >= 0 && page < a.pages;
-    if (lane == 0) {
-      if (ok) {
-        const uint8_t* rec =
-            a.cache + (((int64_t)page * a.kv_heads + ld.h / a.parts) * a.page_tiles + in_page) * L::kRecord;
-        mbar_arrive_expect_tx(&bars[put], L::kRecord);
-        bulk_g2s(ring + put * L::kRecord, rec, L::kRecord, &bars[put]);
-      } else {
-        mbar_arrive(&bars[put]);
-      }
-    }
-    skipped = (skipped & ~(1u << put)) | ((ok ? 0u : 1u) << put);
-    put = put + 1 == ST ? 0 : put + 1;
-    ++ld_x;
-    ++ld.at;
-    if (ld.at >= ld.nt) {
-      settle();
-    } else if (++in_page == a.page_tiles) {
+  auto moved = [&](int n) {  // past n records of this page
+    ld_x += n;
+    ld.at += n;
+    in_page += n;
+    if (src) src += n * L::kRecord;
+    if (in_page == a.page_tiles && ld.at < ld.nt) {
       in_page = 0;
       ++entry;
       page = page_next;
       page_next = a.tables[ld.b * a.table_stride + min(entry + 1, (ld.nt - 1) / a.page_tiles)];
+      find();
     }
+  };
+  auto load = [&] {
+    if (ld_x >= end) return;
+    const int left = min(ld.nt - ld.at, end - ld_x);
+    unsigned char* to = ring + put * P::kStage;
+    uint64_t* bar = &bars[put];
+    bad &= ~(3u << (2 * put));
+    if (left >= 2 && a.page_tiles - in_page >= 2 && src) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, 2 * L::kRecord);
+        bulk_g2s(to, src, 2 * L::kRecord, bar);
+      }
+      moved(2);
+    } else {
+      const uint8_t* from[2] = {src, nullptr};
+      moved(1);
+      if (left >= 2) {
+        from[1] = src;
+        moved(1);
+        if (!from[1]) bad |= 2u << (2 * put);
+      }
+      if (!from[0]) bad |= 1u << (2 * put);
+      if (lane == 0) {
+        const uint32_t bytes = (from[0] ? L::kRecord : 0) + (from[1] ? L::kRecord : 0);
+        if (bytes) {
+          mbar_arrive_expect_tx(bar, bytes);
+          if (from[0]) bulk_g2s(to, from[0], L::kRecord, bar);
+          if (from[1]) bulk_g2s(to + L::kRecord, from[1], L::kRecord, bar);
+        } else {
+          mbar_arrive(bar);
+        }
+      }
+    }
+    put = put + 1 == ST ? 0 : put + 1;
+    if (ld.at >= ld.nt) settle();
   };
   if (x < end && ld.at < ld.nt) enter();
   settle();
@@ -384,7 +416,8 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
 
       float m[NT][2], ref[NT][2], l[NT][2], z[NT][2][NG];
       float o[2 * W][NT][4];
-      float vf = 0x1p100f, back = 0x1p-100f;  // weights enter the product as p scale vf; back = 1 / vf
+      // weights enter the product as p scale vf; back = 1 / vf, scales stay below the limit
+      float vf = 0x1p100f, back = 0x1p-100f, limit = kTopWeight * back;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -401,161 +434,189 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
           for (int c = 0; c < 4; ++c) o[k][n][c] = 0.f;
       }
 
-#pragma unroll 1
-      for (int tile = t0; tile < t1; ++tile) {
-        mbar_wait_nocall(&bars[get], phase);
-        const uint8_t* rec = ring + get * L::kRecord;
-        if (!((skipped >> get) & 1u)) {
-          // scores: tokens g and g + 8 of the record, columns 2 t and 2 t + 1
-          float s[NT][4];
+      // The two records at `rec`, the first of them number `tile`; masked: some row does not
+      // see some token, or there is only one record (bits of `gone`: not there).
+      auto consume = [&](auto masked_type, const uint8_t* rec, int tile, uint32_t gone) {
+        constexpr bool kMasked = decltype(masked_type)::value;
+        // scores: tokens g and g + 8 of a record, columns 2 t and 2 t + 1
+        float s[2][NT][4];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+        for (int i = 0; i < 2; ++i) {
+          uint32_t ka[W], kb[W], pa[NG], pb[NG];
+          const uint8_t* k = rec + i * L::kRecord;
+          load_words(k + g * (D / 2) + t * (D / 8), ka);
+          load_words(k + (g + 8) * (D / 2) + t * (D / 8), kb);
+          load_words(k + L::kKParams + g * (4 * NG), pa);
+          load_words(k + L::kKParams + (g + 8) * (4 * NG), pb);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[n][c] = 0.f;
-          {
-            uint32_t ka[W], kb[W], pa[NG], pb[NG];
-            load_words(rec + g * (D / 2) + t * (D / 8), ka);
-            load_words(rec + (g + 8) * (D / 2) + t * (D / 8), kb);
-            load_words(rec + L::kKParams + g * (4 * NG), pa);
-            load_words(rec + L::kKParams + (g + 8) * (4 * NG), pb);
+          for (int gi = 0; gi < NG; ++gi) {
+            float acc[NT][4];
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi) {
-              float acc[2][NT][4];  // two chains, for the instruction's latency
+            for (int j = 0; j < L::kGroupWords; ++j) {
+              const int w = gi * L::kGroupWords + j;
 #pragma unroll
-              for (int k = 0; k < 2; ++k)
+              for (int q = 0; q < 2; ++q) {
+                const uint32_t u = ka[w] >> (8 * q), v = kb[w] >> (8 * q);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                  for (int c = 0; c < 4; ++c) acc[k][n][c] = 0.f;
-#pragma unroll
-              for (int j = 0; j < L::kGroupWords; ++j) {
-                const int w = gi * L::kGroupWords + j;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const uint32_t u = ka[w] >> (8 * k), v = kb[w] >> (8 * k);
-#pragma unroll
-                  for (int n = 0; n < NT; ++n)
-                    mma_m16n8k16(acc[k][n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
-                                 qf[n][2 * w + k][0], qf[n][2 * w + k][1]);
+                for (int n = 0; n < NT; ++n) {
+                  if (j == 0 && q == 0)
+                    mma_m16n8k16_zero(acc[n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
+                                      qf[n][2 * w + q][0], qf[n][2 * w + q][1]);
+                  else
+                    mma_m16n8k16(acc[n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
+                                 qf[n][2 * w + q][0], qf[n][2 * w + q][1]);
                 }
               }
-              const float2 qa = unpack2<T>(pa[gi]), qb = unpack2<T>(pb[gi]);  // scale, zero
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  s[n][c] = fmaf(qa.x * (acc[0][n][c] + acc[1][n][c]), fac[n][c], fmaf(qa.y, qsum[n][c][gi], s[n][c]));
-                  s[n][2 + c] = fmaf(qb.x * (acc[0][n][2 + c] + acc[1][n][2 + c]), fac[n][c],
-                                     fmaf(qb.y, qsum[n][c][gi], s[n][2 + c]));
-                }
             }
-          }
-          const bool partly = (tile + 1) * kTile > see;  // some row does not see some token
-          if (partly) {
+            const float2 qa = unpack2<T>(pa[gi]), qb = unpack2<T>(pb[gi]);  // scale, zero
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                if (tile * kTile + g >= seen[n][c]) s[n][c] = -INFINITY;
-                if (tile * kTile + g + 8 >= seen[n][c]) s[n][2 + c] = -INFINITY;
+                const float za = gi == 0 ? qa.y * qsum[n][c][gi] : fmaf(qa.y, qsum[n][c][gi], s[i][n][c]);
+                const float zb = gi == 0 ? qb.y * qsum[n][c][gi] : fmaf(qb.y, qsum[n][c][gi], s[i][n][2 + c]);
+                s[i][n][c] = fmaf(qa.x * acc[n][c], fac[n][c], za);
+                s[i][n][2 + c] = fmaf(qb.x * acc[n][2 + c], fac[n][c], zb);
               }
           }
+          if constexpr (kMasked) {
+            const int at = (tile + i) * kTile + g;
+            const bool none = (gone >> i) & 1u;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                if (none || at >= seen[n][c]) s[i][n][c] = -INFINITY;
+                if (none || at + 8 >= seen[n][c]) s[i][n][2 + c] = -INFINITY;
+              }
+          }
+        }
+        float sv[2][2][NG], zv[2][2][NG];  // V's scales x vf and zeros of the lane's tokens
+        float wide = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           uint32_t pa[NG], pb[NG];
-          load_words(rec + L::kVParams + g * (4 * NG), pa);
-          load_words(rec + L::kVParams + (g + 8) * (4 * NG), pb);
-          float sa[NG], sb[NG], za[NG], zb[NG];
-          float wide = 0.f;
-          bool grow = false;
+          load_words(rec + i * L::kRecord + L::kVParams + g * (4 * NG), pa);
+          load_words(rec + i * L::kRecord + L::kVParams + (g + 8) * (4 * NG), pb);
 #pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            const float2 u = unpack2<T>(pa[i]), v = unpack2<T>(pb[i]);
-            sa[i] = u.x, za[i] = u.y, sb[i] = v.x, zb[i] = v.y;
-            if (partly) {  // what lies behind the sequence may be anything
-              if (tile * kTile + g >= len) sa[i] = za[i] = 0.f;
-              if (tile * kTile + g + 8 >= len) sb[i] = zb[i] = 0.f;
+          for (int k = 0; k < NG; ++k) {
+            const float2 u = unpack2<T>(pa[k]), v = unpack2<T>(pb[k]);
+            sv[i][0][k] = u.x, zv[i][0][k] = u.y, sv[i][1][k] = v.x, zv[i][1][k] = v.y;
+            if constexpr (kMasked) {  // what lies behind the sequence may be anything
+              const int at = (tile + i) * kTile + g;
+              const bool none = (gone >> i) & 1u;
+              if (none || at >= len) sv[i][0][k] = zv[i][0][k] = 0.f;
+              if (none || at + 8 >= len) sv[i][1][k] = zv[i][1][k] = 0.f;
             }
-            wide = fmaxf(wide, fmaxf(sa[i], sb[i]));
+            wide = fmaxf(wide, fmaxf(sv[i][0][k], sv[i][1][k]));
           }
-          grow = wide * vf > kTopWeight;
+        }
+        bool grow = wide > limit;
+        float tops[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            tops[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
+            grow = grow || tops[n][c] > m[n][c] + kSlack;
+          }
+        if (__any_sync(kFull, grow)) {
+#pragma unroll
+          for (int k = 4; k < 32; k *= 2) wide = fmaxf(wide, __shfl_xor_sync(kFull, wide, k));
+          float turn = 1.0f;
+          if (wide > limit) {
+            const float now = power_for(wide, 5);
+            turn = now * back;
+            vf = now;
+            back = 1.0f / now;
+            limit = kTopWeight * back;
+          }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) grow = grow || fmaxf(s[n][c], s[n][2 + c]) > m[n][c] + kSlack;
-          if (__any_sync(kFull, grow)) {
+            for (int c = 0; c < 2; ++c) {
+              float top = tops[n][c];
 #pragma unroll
-            for (int k = 4; k < 32; k *= 2) wide = fmaxf(wide, __shfl_xor_sync(kFull, wide, k));
-            float turn = 1.0f;
-            if (wide * vf > kTopWeight) {
-              const float now = power_for(wide, 5);
-              turn = now * back;
-              vf = now;
-              back = 1.0f / now;
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                float top = fmaxf(s[n][c], s[n][2 + c]);
-#pragma unroll
-                for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, k));
-                float f = 1.0f;
-                if (top > m[n][c] + kSlack) {
-                  f = exp2_fast(m[n][c] - top);
-                  m[n][c] = ref[n][c] = top;
-                }
-                l[n][c] *= f;
-#pragma unroll
-                for (int i = 0; i < NG; ++i) z[n][c][i] *= f;
-#pragma unroll
-                for (int k = 0; k < 2 * W; ++k) {
-                  o[k][n][c] *= f * turn;
-                  o[k][n][2 + c] *= f * turn;
-                }
+              for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, k));
+              float f = 1.0f;
+              if (top > m[n][c] + kSlack) {
+                f = exp2_fast(m[n][c] - top);
+                m[n][c] = ref[n][c] = top;
               }
-          }
-          // weights, and weights x scale as operand B of the output's product. What that loses
-          // by its 11 bits is given back for a code of 7.5, the middle of the range: the
-          // codes lie around it, so the error left is that of v's spread and not of its offset.
+              l[n][c] *= f;
+#pragma unroll
+              for (int i = 0; i < NG; ++i) z[n][c][i] *= f;
+#pragma unroll
+              for (int k = 0; k < 2 * W; ++k) {
+                o[k][n][c] *= f * turn;
+                o[k][n][2 + c] *= f * turn;
+              }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // weights, and weights x scale as operand B of the output's product
           uint32_t pf[NT][NG][2];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float p[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) p[c] = exp2_fast(s[n][c] - ref[n][c & 1]);
+            for (int c = 0; c < 4; ++c) p[c] = exp2_fast(s[i][n][c] - ref[n][c & 1]);
             l[n][0] += p[0] + p[2];
             l[n][1] += p[1] + p[3];
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-              float u[4] = {p[0] * (sa[i] * vf), p[1] * (sa[i] * vf), p[2] * (sb[i] * vf), p[3] * (sb[i] * vf)};
-              float y[4] = {p[0] * za[i], p[1] * za[i], p[2] * zb[i], p[3] * zb[i]};
-              if (partly) {  // a token that this row does not see may hold NaN
+            for (int k = 0; k < NG; ++k) {
+              const float sa = sv[i][0][k] * vf, sb = sv[i][1][k] * vf;
+              float u[4] = {p[0] * sa, p[1] * sa, p[2] * sb, p[3] * sb};
+              float zp[4] = {zv[i][0][k], zv[i][0][k], zv[i][1][k], zv[i][1][k]};
+              if constexpr (kMasked) {  // a token that this row does not see may hold NaN
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                  if (s[n][c] == -INFINITY) u[c] = y[c] = 0.f;
+                  if (s[i][n][c] == -INFINITY) u[c] = zp[c] = 0.f;
               }
               const uint32_t ha = half2_bits(u[0], u[1]), hb = half2_bits(u[2], u[3]);
-              const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&ha));
-              const float2 rb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
-              z[n][0][i] += (y[0] + y[2]) + ((u[0] - ra.x) + (u[2] - rb.x)) * (7.5f * back);
-              z[n][1][i] += (y[1] + y[3]) + ((u[1] - ra.y) + (u[3] - rb.y)) * (7.5f * back);
-              pf[n][i][0] = transpose_8x8(ha);
-              pf[n][i][1] = transpose_8x8(hb);
+              z[n][0][k] = fmaf(p[0], zp[0], fmaf(p[2], zp[2], z[n][0][k]));
+              z[n][1][k] = fmaf(p[1], zp[1], fmaf(p[3], zp[3], z[n][1][k]));
+              if constexpr (!Act<T>::kBf16) {
+                // What the 11 bits lose is given back for a code of 7.5, the middle of the
+                // range, so that the error left is that of v's spread and not of its offset:
+                // fp16 outputs would show it (3.5e-4 relative without, 2.4e-4 with), bf16's
+                // own rounding (1.7e-3) hides it.
+                const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&ha));
+                const float2 rb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
+                z[n][0][k] = fmaf((u[0] - ra.x) + (u[2] - rb.x), 7.5f * back, z[n][0][k]);
+                z[n][1][k] = fmaf((u[1] - ra.y) + (u[3] - rb.y), 7.5f * back, z[n][1][k]);
+              }
+              pf[n][k][0] = transpose_8x8(ha);
+              pf[n][k][1] = transpose_8x8(hb);
             }
           }
           uint32_t va[W], vb[W];
-          load_words(rec + L::kV + t * D + ((g ^ (2 * t)) * W) * 4, va);
-          load_words(rec + L::kV + (t + 4) * D + ((g ^ (2 * t)) * W) * 4, vb);
+          const uint8_t* v = rec + i * L::kRecord + L::kV + t * D + ((g ^ (2 * t)) * W) * 4;
+          load_words(v, va);
+          load_words(v + 4 * D, vb);
 #pragma unroll
           for (int w = 0; w < W; ++w)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const uint32_t u = va[w] >> (8 * k), v = vb[w] >> (8 * k);
+              const uint32_t u = va[w] >> (8 * k), y = vb[w] >> (8 * k);
 #pragma unroll
               for (int n = 0; n < NT; ++n)
-                mma_m16n8k16(o[2 * w + k][n], u & 0x000f000fu, u & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u,
+                mma_m16n8k16(o[2 * w + k][n], u & 0x000f000fu, u & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u,
                              pf[n][w / L::kGroupWords][0], pf[n][w / L::kGroupWords][1]);
             }
         }
+      };
+      const int clear = min(t1, see / kTile);  // records before this one are seen whole by all rows
+#pragma unroll 1
+      for (int tile = t0; tile < t1; tile += 2) {
+        mbar_wait_nocall(&bars[get], phase);
+        const uint8_t* rec = ring + get * P::kStage;
+        uint32_t gone = (bad >> (2 * get)) & 3u;
+        if (tile + 2 <= clear && gone == 0)
+          consume(std::false_type{}, rec, tile, 0u);
+        else
+          consume(std::true_type{}, rec, tile, tile + 1 < t1 ? gone : gone | 2u);
         __syncwarp();
         load();
         if (++get == ST) {
