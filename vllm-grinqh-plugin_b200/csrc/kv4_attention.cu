@@ -35,8 +35,8 @@ namespace grinqh {
 namespace {
 
 constexpr int kMaxRows = 32;  // new tokens x query heads of a kv head
-constexpr float kSlack = 8.0f;       // weights may reach 2^kSlack before the running maximum follows
-constexpr float kTopWeight = 64.0f;  // V scales x vf stay below this, weights x that in f16's range
+constexpr float kSlack = 1024.0f;  // a lane's weights of a step may sum to this before the maximum follows
+constexpr int kTopScale = 4;       // V scales x vf stay below 2^(kTopScale + 1): weights x that within f16's range
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr uint32_t kFull = 0xffffffffu;
 
@@ -72,7 +72,7 @@ struct Plan {
   static constexpr uint32_t kWarpRing = kStages * kStage;
   static constexpr uint32_t kSmem = kWarps * (kWarpRing + kSums * 4 + kStages * 8) + 512;
   // as many as 228 KB of shared memory and the registers let an SM hold
-  static constexpr int kCtas = NT == 2 && 3 * (kSmem + 1024) <= 233472 ? 3 : 2;
+  static constexpr int kCtas = NT == 2 && D == 64 ? 3 : 2;
   static_assert(kSums * 4 <= kWarpRing, "a run's last sums go where its ring was");
   static_assert(kCtas * (kSmem + 1024) <= 233472, "shared memory");
 };
@@ -252,87 +252,90 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
 
   // ---------------------------------------------------------------- the warp's loads
   // A stage takes the next two records of a sequence and head (the last of them alone may
-  // be one): one copy where they lie in one page. Page numbers are read a page ahead.
-  int ld_x = x, put = 0;  // place of the next record to load; stage it goes to
+  // be one): one copy where they lie in one page. `ready` records from src on lie in one
+  // page and belong to the run; `ld` and `ld_x` are the place behind them. Page numbers are
+  // read a page ahead.
+  int ld_x = x, ready = 0;
   Pos ld = seg;
-  int page = 0, page_next = 0, in_page = 0, entry = 0;
-  const uint8_t* src = nullptr;
-  uint32_t bad = 0;  // two bits per stage: record of a page outside the cache, not loaded
-  auto find = [&] {  // the record at in_page of `page`
+  int page = 0, page_next = 0, entry = 0;
+  const uint8_t* src = nullptr;  // null: a page outside the cache, nothing is loaded
+  uint32_t bad = 0;              // two bits per stage: record that was not loaded
+  auto gather = [&](int in_page) {  // the records from in_page of `page` on
+    ready = min(min(a.page_tiles - in_page, ld.nt - ld.at), end - ld_x);
     src = page >= 0 && page < a.pages
               ? a.cache + (((int64_t)page * a.kv_heads + ld.h / a.parts) * a.page_tiles + in_page) * L::kRecord
               : nullptr;
+    ld.at += ready;
+    ld_x += ready;
   };
-  auto enter = [&] {  // a sequence and head
-    entry = ld.at / a.page_tiles;
-    in_page = ld.at - entry * a.page_tiles;
-    const int32_t* table = a.tables + ld.b * a.table_stride;
-    page = table[entry];
-    page_next = table[min(entry + 1, (ld.nt - 1) / a.page_tiles)];
-    find();
-  };
-  auto settle = [&] {  // from a place that is no record to the next one that is
-    while (ld_x < end && ld.at >= ld.nt) {
-      const int step = ld.stride - ld.at;
-      ld_x += step;
-      if (ld_x < end) {
-        advance(a, ld, step, same);
-        enter();
-      }
-    }
-  };
-  auto moved = [&](int n) {  // past n records of this page
-    ld_x += n;
-    ld.at += n;
-    in_page += n;
-    if (src) src += n * L::kRecord;
-    if (in_page == a.page_tiles && ld.at < ld.nt) {
-      in_page = 0;
+  auto more = [&] {  // the next records, ready being 0
+    if (ld_x >= end) return;
+    if (ld.at > 0 && ld.at < ld.nt) {
       ++entry;
       page = page_next;
       page_next = a.tables[ld.b * a.table_stride + min(entry + 1, (ld.nt - 1) / a.page_tiles)];
-      find();
+      gather(0);
+      return;
     }
+    while (ld.at >= ld.nt) {  // to the next place that is a record
+      const int step = ld.stride - ld.at;
+      ld_x += step;
+      if (ld_x >= end) return;
+      advance(a, ld, step, same);
+    }
+    const int32_t* table = a.tables + ld.b * a.table_stride;
+    page = table[0];
+    page_next = table[min(1, (ld.nt - 1) / a.page_tiles)];
+    entry = 0;
+    gather(0);
   };
-  auto load = [&] {
-    if (ld_x >= end) return;
-    const int left = min(ld.nt - ld.at, end - ld_x);
-    unsigned char* to = ring + put * P::kStage;
-    uint64_t* bar = &bars[put];
-    bad &= ~(3u << (2 * put));
-    if (left >= 2 && a.page_tiles - in_page >= 2 && src) {
+  auto load = [&](int stage) {
+    if (ready == 0) return;  // the run is at its end
+    unsigned char* to = ring + stage * P::kStage;
+    uint64_t* bar = &bars[stage];
+    if (ready >= 2 && src) {
       if (lane == 0) {
-        mbar_arrive_expect_tx(bar, 2 * L::kRecord);
-        bulk_g2s(to, src, 2 * L::kRecord, bar);
+        mbar_arrive_expect_tx(bar, P::kStage);
+        bulk_g2s(to, src, P::kStage, bar);
       }
-      moved(2);
+      src += P::kStage;
+      ready -= 2;
+      bad &= ~(3u << (2 * stage));
     } else {
-      const uint8_t* from[2] = {src, nullptr};
-      moved(1);
-      if (left >= 2) {
-        from[1] = src;
-        moved(1);
-        if (!from[1]) bad |= 2u << (2 * put);
+      const bool two = ready >= 2 || ld.at < ld.nt && ld_x < end;  // a second record in this sequence and head
+      const uint8_t *first = src, *second = nullptr;
+      if (src) src += L::kRecord;
+      if (--ready == 0) more();
+      if (two) {
+        second = src;
+        if (src) src += L::kRecord;
+        --ready;
       }
-      if (!from[0]) bad |= 1u << (2 * put);
+      bad = (bad & ~(3u << (2 * stage))) | ((first ? 0u : 1u) | (two && !second ? 2u : 0u)) << (2 * stage);
       if (lane == 0) {
-        const uint32_t bytes = (from[0] ? L::kRecord : 0) + (from[1] ? L::kRecord : 0);
+        const uint32_t bytes = (first ? L::kRecord : 0) + (second ? L::kRecord : 0);
         if (bytes) {
           mbar_arrive_expect_tx(bar, bytes);
-          if (from[0]) bulk_g2s(to, from[0], L::kRecord, bar);
-          if (from[1]) bulk_g2s(to + L::kRecord, from[1], L::kRecord, bar);
+          if (first) bulk_g2s(to, first, L::kRecord, bar);
+          if (second) bulk_g2s(to + L::kRecord, second, L::kRecord, bar);
         } else {
           mbar_arrive(bar);
         }
       }
     }
-    put = put + 1 == ST ? 0 : put + 1;
-    if (ld.at >= ld.nt) settle();
+    if (ready == 0) more();
   };
-  if (x < end && ld.at < ld.nt) enter();
-  settle();
+  if (x < end && ld.at > 0 && ld.at < ld.nt) {  // into the middle of a sequence and head
+    entry = ld.at / a.page_tiles;
+    const int32_t* table = a.tables + ld.b * a.table_stride;
+    page = table[entry];
+    page_next = table[min(entry + 1, (ld.nt - 1) / a.page_tiles)];
+    gather(ld.at - entry * a.page_tiles);
+  } else {
+    more();
+  }
 #pragma unroll 1
-  for (int s = 0; s < ST; ++s) load();
+  for (int s = 0; s < ST; ++s) load(s);
 
   // One row of a finished sequence and head: 4 channels from d on.
   auto finish = [&](int b, int h, int r, int d, float top, float sum, float4 v) {
@@ -417,7 +420,8 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
       float m[NT][2], ref[NT][2], l[NT][2], z[NT][2][NG];
       float o[2 * W][NT][4];
       // weights enter the product as p scale vf; back = 1 / vf, scales stay below the limit
-      float vf = 0x1p100f, back = 0x1p-100f, limit = kTopWeight * back;
+      float vf = 0x1p100f, back = 0x1p-100f, limit = (float)(2 << kTopScale) * back;
+      bool first = true;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -440,46 +444,54 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
         constexpr bool kMasked = decltype(masked_type)::value;
         // scores: tokens g and g + 8 of a record, columns 2 t and 2 t + 1
         float s[2][NT][4];
+        uint32_t ka[2][W], kb[2][W], pa[2][NG], pb[2][NG];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t ka[W], kb[W], pa[NG], pb[NG];
           const uint8_t* k = rec + i * L::kRecord;
-          load_words(k + g * (D / 2) + t * (D / 8), ka);
-          load_words(k + (g + 8) * (D / 2) + t * (D / 8), kb);
-          load_words(k + L::kKParams + g * (4 * NG), pa);
-          load_words(k + L::kKParams + (g + 8) * (4 * NG), pb);
+          load_words(k + g * (D / 2) + t * (D / 8), ka[i]);
+          load_words(k + (g + 8) * (D / 2) + t * (D / 8), kb[i]);
+          load_words(k + L::kKParams + g * (4 * NG), pa[i]);
+          load_words(k + L::kKParams + (g + 8) * (4 * NG), pb[i]);
+        }
 #pragma unroll
-          for (int gi = 0; gi < NG; ++gi) {
-            float acc[NT][4];
+        for (int gi = 0; gi < NG; ++gi) {
+          float acc[2][NT][4];
 #pragma unroll
-            for (int j = 0; j < L::kGroupWords; ++j) {
-              const int w = gi * L::kGroupWords + j;
+          for (int j = 0; j < L::kGroupWords; ++j) {
+            const int w = gi * L::kGroupWords + j;
 #pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const uint32_t u = ka[w] >> (8 * q), v = kb[w] >> (8 * q);
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t u = ka[i][w] >> (8 * q), v = kb[i][w] >> (8 * q);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                   if (j == 0 && q == 0)
-                    mma_m16n8k16_zero(acc[n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
+                    mma_m16n8k16_zero(acc[i][n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
                                       qf[n][2 * w + q][0], qf[n][2 * w + q][1]);
                   else
-                    mma_m16n8k16(acc[n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
+                    mma_m16n8k16(acc[i][n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
                                  qf[n][2 * w + q][0], qf[n][2 * w + q][1]);
                 }
               }
-            }
-            const float2 qa = unpack2<T>(pa[gi]), qb = unpack2<T>(pb[gi]);  // scale, zero
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 qa = unpack2<T>(pa[i][gi]), qb = unpack2<T>(pb[i][gi]);  // scale, zero
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 const float za = gi == 0 ? qa.y * qsum[n][c][gi] : fmaf(qa.y, qsum[n][c][gi], s[i][n][c]);
                 const float zb = gi == 0 ? qb.y * qsum[n][c][gi] : fmaf(qb.y, qsum[n][c][gi], s[i][n][2 + c]);
-                s[i][n][c] = fmaf(qa.x * acc[n][c], fac[n][c], za);
-                s[i][n][2 + c] = fmaf(qb.x * acc[n][2 + c], fac[n][c], zb);
+                s[i][n][c] = fmaf(qa.x * acc[i][n][c], fac[n][c], za);
+                s[i][n][2 + c] = fmaf(qb.x * acc[i][n][2 + c], fac[n][c], zb);
               }
           }
-          if constexpr (kMasked) {
+        }
+        if constexpr (kMasked) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
             const int at = (tile + i) * kTile + g;
             const bool none = (gone >> i) & 1u;
 #pragma unroll
@@ -491,16 +503,16 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
               }
           }
         }
-        float sv[2][2][NG], zv[2][2][NG];  // V's scales x vf and zeros of the lane's tokens
+        // V's scales and zeros of the lane's tokens
+        float sv[2][2][NG], zv[2][2][NG];
         float wide = 0.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t pa[NG], pb[NG];
-          load_words(rec + i * L::kRecord + L::kVParams + g * (4 * NG), pa);
-          load_words(rec + i * L::kRecord + L::kVParams + (g + 8) * (4 * NG), pb);
+          load_words(rec + i * L::kRecord + L::kVParams + g * (4 * NG), pa[i]);
+          load_words(rec + i * L::kRecord + L::kVParams + (g + 8) * (4 * NG), pb[i]);
 #pragma unroll
           for (int k = 0; k < NG; ++k) {
-            const float2 u = unpack2<T>(pa[k]), v = unpack2<T>(pb[k]);
+            const float2 u = unpack2<T>(pa[i][k]), v = unpack2<T>(pb[i][k]);
             sv[i][0][k] = u.x, zv[i][0][k] = u.y, sv[i][1][k] = v.x, zv[i][1][k] = v.y;
             if constexpr (kMasked) {  // what lies behind the sequence may be anything
               const int at = (tile + i) * kTile + g;
@@ -511,38 +523,49 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
             wide = fmaxf(wide, fmaxf(sv[i][0][k], sv[i][1][k]));
           }
         }
-        bool grow = wide > limit;
-        float tops[NT][2];
+        // Weights by the maximum so far. Where they sum to more than kSlack the maximum is
+        // raised and they are made anew; `first` makes that so until every row has a maximum.
+        float p[2][NT][4], add[NT][2];
+        auto weigh = [&] {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            tops[n][c] = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
-            grow = grow || tops[n][c] > m[n][c] + kSlack;
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) p[i][n][c] = exp2_fast(s[i][n][c] - ref[n][c & 1]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) add[n][c] = (p[0][n][c] + p[0][n][2 + c]) + (p[1][n][c] + p[1][n][2 + c]);
           }
+        };
+        weigh();
+        bool grow = first || wide > limit;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) grow = grow || fmaxf(add[n][0], add[n][1]) > kSlack;
         if (__any_sync(kFull, grow)) {
+          bool unset = false;
 #pragma unroll
           for (int k = 4; k < 32; k *= 2) wide = fmaxf(wide, __shfl_xor_sync(kFull, wide, k));
           float turn = 1.0f;
           if (wide > limit) {
-            const float now = power_for(wide, 5);
+            const float now = power_for(wide, kTopScale);
             turn = now * back;
             vf = now;
             back = 1.0f / now;
-            limit = kTopWeight * back;
+            limit = (float)(2 << kTopScale) * back;
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              float top = tops[n][c];
+              float top = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
 #pragma unroll
               for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, k));
               float f = 1.0f;
-              if (top > m[n][c] + kSlack) {
+              if (top > m[n][c]) {
                 f = exp2_fast(m[n][c] - top);
                 m[n][c] = ref[n][c] = top;
               }
+              unset = unset || m[n][c] == -INFINITY;
               l[n][c] *= f;
 #pragma unroll
               for (int i = 0; i < NG; ++i) z[n][c][i] *= f;
@@ -552,22 +575,24 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
                 o[k][n][2 + c] *= f * turn;
               }
             }
+          first = __any_sync(kFull, unset);
+          weigh();
         }
 #pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) l[n][c] += add[n][c];
+#pragma unroll
         for (int i = 0; i < 2; ++i) {
-          // weights, and weights x scale as operand B of the output's product
+          // weights x scale as operand B of the output's product
           uint32_t pf[NT][NG][2];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float p[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) p[c] = exp2_fast(s[i][n][c] - ref[n][c & 1]);
-            l[n][0] += p[0] + p[2];
-            l[n][1] += p[1] + p[3];
+            const float* w = p[i][n];
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
               const float sa = sv[i][0][k] * vf, sb = sv[i][1][k] * vf;
-              float u[4] = {p[0] * sa, p[1] * sa, p[2] * sb, p[3] * sb};
+              float u[4] = {w[0] * sa, w[1] * sa, w[2] * sb, w[3] * sb};
               float zp[4] = {zv[i][0][k], zv[i][0][k], zv[i][1][k], zv[i][1][k]};
               if constexpr (kMasked) {  // a token that this row does not see may hold NaN
 #pragma unroll
@@ -575,8 +600,8 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
                   if (s[i][n][c] == -INFINITY) u[c] = zp[c] = 0.f;
               }
               const uint32_t ha = half2_bits(u[0], u[1]), hb = half2_bits(u[2], u[3]);
-              z[n][0][k] = fmaf(p[0], zp[0], fmaf(p[2], zp[2], z[n][0][k]));
-              z[n][1][k] = fmaf(p[1], zp[1], fmaf(p[3], zp[3], z[n][1][k]));
+              z[n][0][k] = fmaf(w[0], zp[0], fmaf(w[2], zp[2], z[n][0][k]));
+              z[n][1][k] = fmaf(w[1], zp[1], fmaf(w[3], zp[3], z[n][1][k]));
               if constexpr (!Act<T>::kBf16) {
                 // What the 11 bits lose is given back for a code of 7.5, the middle of the
                 // range, so that the error left is that of v's spread and not of its offset:
@@ -595,34 +620,45 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
           const uint8_t* v = rec + i * L::kRecord + L::kV + t * D + ((g ^ (2 * t)) * W) * 4;
           load_words(v, va);
           load_words(v + 4 * D, vb);
+          // Rows g are fed the whole byte 16 hi + lo, rows g + 8 its 16 hi: their difference
+          // in the end is lo's sum, exact but for fp32's rounding, and an AND fewer per word.
 #pragma unroll
           for (int w = 0; w < W; ++w)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const uint32_t u = va[w] >> (8 * k), y = vb[w] >> (8 * k);
+              const uint32_t u = k == 0 ? va[w] & 0x00ff00ffu : __byte_perm(va[w], 0u, 0x4341u);
+              const uint32_t y = k == 0 ? vb[w] & 0x00ff00ffu : __byte_perm(vb[w], 0u, 0x4341u);
 #pragma unroll
               for (int n = 0; n < NT; ++n)
-                mma_m16n8k16(o[2 * w + k][n], u & 0x000f000fu, u & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u,
-                             pf[n][w / L::kGroupWords][0], pf[n][w / L::kGroupWords][1]);
+                mma_m16n8k16(o[2 * w + k][n], u, u & 0x00f000f0u, y, y & 0x00f000f0u, pf[n][w / L::kGroupWords][0],
+                             pf[n][w / L::kGroupWords][1]);
             }
         }
       };
       const int clear = min(t1, see / kTile);  // records before this one are seen whole by all rows
-#pragma unroll 1
-      for (int tile = t0; tile < t1; tile += 2) {
-        mbar_wait_nocall(&bars[get], phase);
-        const uint8_t* rec = ring + get * P::kStage;
-        uint32_t gone = (bad >> (2 * get)) & 3u;
-        if (tile + 2 <= clear && gone == 0)
-          consume(std::false_type{}, rec, tile, 0u);
-        else
-          consume(std::true_type{}, rec, tile, tile + 1 < t1 ? gone : gone | 2u);
+      auto release = [&] {
         __syncwarp();
-        load();
+        load(get);
         if (++get == ST) {
           get = 0;
           phase ^= 1;
         }
+      };
+      // a loop of its own for the records that need no mask: a choice in each step would
+      // have the sums moved between registers (28 % more instructions)
+      for (int tile = t0; tile < t1;) {
+#pragma unroll 1
+        for (; tile + 2 <= clear && ((bad >> (2 * get)) & 3u) == 0; tile += 2) {
+          mbar_wait_nocall(&bars[get], phase);
+          consume(std::false_type{}, ring + get * P::kStage, tile, 0u);
+          release();
+        }
+        if (tile >= t1) break;
+        const uint32_t gone = (bad >> (2 * get)) & 3u;
+        mbar_wait_nocall(&bars[get], phase);
+        consume(std::true_type{}, ring + get * P::kStage, tile, tile + 1 < t1 ? gone : gone | 2u);
+        release();
+        tile += 2;
       }
 
       // ---------------------------------------------------------- the piece's sums
@@ -648,9 +684,9 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
             const int gi = w / L::kGroupWords, j = w % L::kGroupWords;
             const int d = gi * GS + g * (GS / 8) + 4 * j;
             const float f = back * 16777216.0f;
-            const float4 v = make_float4(fmaf(o[2 * w][n][c], f, z[n][c][gi]),
+            const float4 v = make_float4(fmaf(o[2 * w][n][c] - o[2 * w][n][2 + c], f, z[n][c][gi]),
                                          fmaf(o[2 * w][n][2 + c], f * 0.0625f, z[n][c][gi]),
-                                         fmaf(o[2 * w + 1][n][c], f, z[n][c][gi]),
+                                         fmaf(o[2 * w + 1][n][c] - o[2 * w + 1][n][2 + c], f, z[n][c][gi]),
                                          fmaf(o[2 * w + 1][n][2 + c], f * 0.0625f, z[n][c][gi]));
             if (began || goes) {
               *reinterpret_cast<float4*>(sums + r * P::kRow + d) = v;
