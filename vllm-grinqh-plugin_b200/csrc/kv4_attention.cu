@@ -19,11 +19,13 @@
 // times the bytes written and read there for an instruction of at least 64 rows.
 //
 // Work is cut evenly: the records (16 tokens) of all sequences and kv heads are numbered
-// in a row, and every warp takes a run of them, streamed through its own ring of bulk
-// copies across the borders of sequences. A sequence and head that lies in one run is
-// finished by its warp; the sums of one that several warps share are joined in shared
-// memory when the CTA's warps are done, and where it is shared by several CTAs, each
-// writes its sums to the workspace and the last one to arrive joins them in order.
+// in a row, and every warp takes a run of them, which streams through a ring of its own
+// across the borders of sequences. One warp issues the bulk copies for all rings, a lane
+// each: looking up pages would cost the computing warps a quarter more instructions and
+// the registers that keep two records in flight. A sequence and head that lies in one
+// run is finished by its warp; the sums of one that several warps share are joined in
+// shared memory when the CTA's warps are done, and where it is shared by several CTAs,
+// each writes its sums to the workspace and the last one to arrive joins them in order.
 #include "kv4.cuh"
 #include "kv4_attention.cuh"
 #include "ptx.cuh"
@@ -49,6 +51,7 @@ struct Kv4AttnArgs {
   void* out;
   float* lse;
   float* slots;       // [CTA][2]{m, l of the rows, O[rows][D]}: sums of a shared sequence and head
+  float* sums;        // [CTA][warp]{O, m, l}: of a piece that began before the warp's run
   unsigned* tickets;  // [CTA]: arrivals for the one that begins in this CTA and goes on
   int64_t table_stride;
   int64_t pages;
@@ -62,24 +65,23 @@ struct Kv4AttnArgs {
 template <int D, int GS, int NT>
 struct Plan {
   static constexpr int kRows = 8 * NT;
-  // 8 warps, or as many as keep two CTAs on an SM
-  static constexpr int kWarps = NT == 2 ? 4 : (D == 128 && GS == 32 ? 6 : 8);
-  static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kStages = D == 64 ? 3 : 2;        // of two records each
+  // Warps that compute, beside the one that loads: one CTA per SM, and 128 registers a
+  // thread, or 255 where the sums of 16 rows x 128 channels take 128 of them.
+  static constexpr int kWarps = NT == 2 && D == 128 ? 7 : (D == 128 && GS == 32 ? 14 : 15);
+  static constexpr int kThreads = 32 * (kWarps + 1);
+  // Stages of two records.
+  static constexpr int kStages = D == 64 ? 5 : 3;
   static constexpr uint32_t kStage = 2 * Kv4<D, GS>::kRecord;
-  static constexpr int kRow = D + 4;                     // floats of a row of sums in shared memory
+  static constexpr int kRow = D + 4;                     // floats of a row of sums
   static constexpr int kSums = kRows * kRow + 2 * kRows;  // O, m, l
   static constexpr uint32_t kWarpRing = kStages * kStage;
-  static constexpr uint32_t kSmem = kWarps * (kWarpRing + kSums * 4 + kStages * 8) + 512;
-  // as many as 228 KB of shared memory and the registers let an SM hold
-  static constexpr int kCtas = NT == 2 && D == 64 ? 3 : 2;
+  static constexpr uint32_t kSmem = kWarps * kWarpRing;
   static_assert(kSums * 4 <= kWarpRing, "a run's last sums go where its ring was");
-  static_assert(kCtas * (kSmem + 1024) <= 233472, "shared memory");
+  static_assert(kSmem <= 225 * 1024, "shared memory");
 };
 
-constexpr int kMaxCtas = 3;  // per SM
 // What a sequence and head costs beside its records, in records: q, finishing or joining.
-constexpr int kCost = 6;
+constexpr int kCost = 8;
 
 __device__ __forceinline__ int tiles_of(const Kv4AttnArgs& a, int b) {
   return (min(max(a.lens[b], 0), a.max_len) + kTile - 1) / kTile;
@@ -109,7 +111,9 @@ __device__ __forceinline__ void advance(const Kv4AttnArgs& a, Pos& p, int step, 
 
 // What a warp leaves to join: a piece of a sequence and head that began before its run
 // (kHead; kThrough if it also goes on behind it), and one that goes on behind it (kTail).
-enum { kHead = 1, kThrough = 2, kTail = 4 };
+// The sums of the run's last piece are in the ring, those of a head before it in the
+// workspace (kAway).
+enum { kHead = 1, kThrough = 2, kTail = 4, kAway = 8 };
 struct Piece {
   int b, h, first, nt;  // first: the place of its first record
 };
@@ -126,6 +130,14 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+template <typename T>
+__device__ __forceinline__ auto two(uint32_t w) {
+  if constexpr (Act<T>::kBf16)
+    return *reinterpret_cast<const __nv_bfloat162*>(&w);
+  else
+    return *reinterpret_cast<const __half2*>(&w);
+}
+
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -135,6 +147,19 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 __device__ __forceinline__ float power_for(float x, int e) {
   const int ex = (int)(__float_as_uint(x) >> 23) - 127;
   return __uint_as_float((uint32_t)(min(max(e - ex, -126), 127) + 127) << 23);
+}
+
+// Adds sums l, y by the maximum m to those by `top`.
+__device__ __forceinline__ void add_sums(float& top, float& sum, float4& v, float m, float l, float4 y) {
+  const bool some = l != 0.f;  // (a NaN counts)
+  const float now = some ? fmaxf(top, m) : top;
+  const float f = now == -INFINITY ? 1.0f : exp2_fast(top - now), h = some ? exp2_fast(m - now) : 0.f;
+  top = now;
+  sum = fmaf(l, h, sum * f);
+  v.x = some ? fmaf(y.x, h, v.x * f) : v.x;
+  v.y = some ? fmaf(y.y, h, v.y * f) : v.y;
+  v.z = some ? fmaf(y.z, h, v.z * f) : v.z;
+  v.w = some ? fmaf(y.w, h, v.w * f) : v.w;
 }
 
 template <int N>
@@ -151,14 +176,16 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
 }
 
 template <typename T, int D, int GS, int NT>
-__global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kCtas)
-    kv4_attention_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_kernel(const Kv4AttnArgs a) {
   using L = Kv4<D, GS>;
   using P = Plan<D, GS, NT>;
+  using T2 = decltype(two<T>(0u));
   constexpr int NG = L::NG, W = L::kWords, NW = P::kWarps, ST = P::kStages;
   extern __shared__ __align__(128) unsigned char smem[];
-  float* s_sums = reinterpret_cast<float*>(smem + NW * P::kWarpRing);
-  uint64_t* s_bars = reinterpret_cast<uint64_t*>(s_sums + NW * P::kSums);
+  float* heads_of = a.sums + (int64_t)blockIdx.x * NW * P::kSums;  // of the warps: pieces that began before
+  __shared__ uint64_t s_full[NW][ST], s_empty[NW][ST];
+  __shared__ uint32_t s_gone[NW][ST];  // bits: record of the stage that was not loaded
+  __shared__ int s_pages[NW][64];
   __shared__ Pos s_start;
   __shared__ int s_plan[3];  // places of a run, the common stride (0: none), places in all
   __shared__ Left s_left[NW];
@@ -167,16 +194,17 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int heads = a.kv_heads * a.parts;  // what is numbered within a sequence
-  uint64_t* bars = s_bars + warp * ST;
-  unsigned char* ring = smem + warp * P::kWarpRing;
-  if (lane == 0) {
-    for (int s = 0; s < ST; ++s) mbar_init(&bars[s], 1);
+  if (warp < NW && lane == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&s_full[warp][s], 1);
+      mbar_init(&s_empty[warp][s], 1);
+    }
     fence_mbar_init();
     s_left[warp].flags = 0;
   }
 
   // ---------------------------------------------------------------- the CTA's runs
-  if (warp == 0) {
+  if (warp == NW) {
     int tiles = 0, most = 0, count = 0;
     for (int b = lane; b < a.seqs; b += 32) {
       const int n = tiles_of(a, b);
@@ -237,109 +265,20 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
     for (int b = blockIdx.x; b < a.seqs; b += gridDim.x) {
       if (tiles_of(a, b) > 0) continue;
       const int64_t at = (int64_t)b * a.fresh * a.heads;
-      for (int64_t i = threadIdx.x - 32; i < (int64_t)a.fresh * a.heads * (D / 8); i += P::kThreads - 32)
+      for (int64_t i = threadIdx.x; i < (int64_t)a.fresh * a.heads * (D / 8); i += 32 * NW)
         reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at * D)[i] = make_uint4(0u, 0u, 0u, 0u);
-      for (int i = threadIdx.x - 32; i < a.fresh * a.heads; i += P::kThreads - 32) a.lse[at + i] = -INFINITY;
+      for (int i = threadIdx.x; i < a.fresh * a.heads; i += 32 * NW) a.lse[at + i] = -INFINITY;
     }
   }
   __syncthreads();
   const int per = s_plan[0], same = s_plan[1], total = s_plan[2];
   if ((int)blockIdx.x * NW * per >= total) return;
   Pos seg = s_start;
-  int x = ((int)blockIdx.x * NW + warp) * per;  // this warp's run: places x .. end
-  const int end = min(x + per, total);
-  if (x < end) advance(a, seg, warp * per, same);
-
-  // ---------------------------------------------------------------- the warp's loads
-  // A stage takes the next two records of a sequence and head (the last of them alone may
-  // be one): one copy where they lie in one page. `ready` records from src on lie in one
-  // page and belong to the run; `ld` and `ld_x` are the place behind them. Page numbers are
-  // read a page ahead.
-  int ld_x = x, ready = 0;
-  Pos ld = seg;
-  int page = 0, page_next = 0, entry = 0;
-  const uint8_t* src = nullptr;  // null: a page outside the cache, nothing is loaded
-  uint32_t bad = 0;              // two bits per stage: record that was not loaded
-  auto gather = [&](int in_page) {  // the records from in_page of `page` on
-    ready = min(min(a.page_tiles - in_page, ld.nt - ld.at), end - ld_x);
-    src = page >= 0 && page < a.pages
-              ? a.cache + (((int64_t)page * a.kv_heads + ld.h / a.parts) * a.page_tiles + in_page) * L::kRecord
-              : nullptr;
-    ld.at += ready;
-    ld_x += ready;
-  };
-  auto more = [&] {  // the next records, ready being 0
-    if (ld_x >= end) return;
-    if (ld.at > 0 && ld.at < ld.nt) {
-      ++entry;
-      page = page_next;
-      page_next = a.tables[ld.b * a.table_stride + min(entry + 1, (ld.nt - 1) / a.page_tiles)];
-      gather(0);
-      return;
-    }
-    while (ld.at >= ld.nt) {  // to the next place that is a record
-      const int step = ld.stride - ld.at;
-      ld_x += step;
-      if (ld_x >= end) return;
-      advance(a, ld, step, same);
-    }
-    const int32_t* table = a.tables + ld.b * a.table_stride;
-    page = table[0];
-    page_next = table[min(1, (ld.nt - 1) / a.page_tiles)];
-    entry = 0;
-    gather(0);
-  };
-  auto load = [&](int stage) {
-    if (ready == 0) return;  // the run is at its end
-    unsigned char* to = ring + stage * P::kStage;
-    uint64_t* bar = &bars[stage];
-    if (ready >= 2 && src) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar, P::kStage);
-        bulk_g2s(to, src, P::kStage, bar);
-      }
-      src += P::kStage;
-      ready -= 2;
-      bad &= ~(3u << (2 * stage));
-    } else {
-      const bool two = ready >= 2 || ld.at < ld.nt && ld_x < end;  // a second record in this sequence and head
-      const uint8_t *first = src, *second = nullptr;
-      if (src) src += L::kRecord;
-      if (--ready == 0) more();
-      if (two) {
-        second = src;
-        if (src) src += L::kRecord;
-        --ready;
-      }
-      bad = (bad & ~(3u << (2 * stage))) | ((first ? 0u : 1u) | (two && !second ? 2u : 0u)) << (2 * stage);
-      if (lane == 0) {
-        const uint32_t bytes = (first ? L::kRecord : 0) + (second ? L::kRecord : 0);
-        if (bytes) {
-          mbar_arrive_expect_tx(bar, bytes);
-          if (first) bulk_g2s(to, first, L::kRecord, bar);
-          if (second) bulk_g2s(to + L::kRecord, second, L::kRecord, bar);
-        } else {
-          mbar_arrive(bar);
-        }
-      }
-    }
-    if (ready == 0) more();
-  };
-  if (x < end && ld.at > 0 && ld.at < ld.nt) {  // into the middle of a sequence and head
-    entry = ld.at / a.page_tiles;
-    const int32_t* table = a.tables + ld.b * a.table_stride;
-    page = table[entry];
-    page_next = table[min(entry + 1, (ld.nt - 1) / a.page_tiles)];
-    gather(ld.at - entry * a.page_tiles);
-  } else {
-    more();
-  }
-#pragma unroll 1
-  for (int s = 0; s < ST; ++s) load(s);
 
   // One row of a finished sequence and head: 4 channels from d on.
   auto finish = [&](int b, int h, int r, int d, float top, float sum, float4 v) {
-    const int64_t row = ((int64_t)b * a.fresh + r / a.group) * a.heads + h * a.group + r % a.group;
+    const int j = a.fresh == 1 ? 0 : r / a.group;
+    const int64_t row = ((int64_t)b * a.fresh + j) * a.heads + h * a.group + r - j * a.group;
     const bool none = sum == 0.f;
     const float inv = 1.0f / sum;
     const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
@@ -350,365 +289,465 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
     if (d == 0) a.lse[row] = none ? -INFINITY : (top + log2f(sum)) * kLn2;
   };
 
-  int get = 0, phase = 0;  // consuming: stage, parity
-  // ---------------------------------------------------------------- piece by piece
-  while (x < end) {
-    const int t0 = seg.at, t1 = min(seg.nt, seg.at + (end - x));  // this piece's records
-    if (t0 < t1) {
-      const int kv_head = seg.h / a.parts, row0 = (seg.h - kv_head * a.parts) * P::kRows;
-      const int rows = min(a.fresh * a.group - row0, P::kRows);
-      const int len = min(max(a.lens[seg.b], 0), a.max_len);
-      const int see = len - a.fresh + 1 + row0 / a.group;  // tokens that the first row sees
-
-      // q as operand B: column g of block n is query row 8 n + g; this lane's channels are
-      // those of chunk t of a K row. f16 with the row's largest value near 2^13, so that the
-      // half of them that is divided by 16 keeps its bits; below 2^-22 of the largest they
-      // are rounded, which moves no score by more than 2^-24 of its largest term.
-      uint32_t qf[NT][D / 16][2];
-      float fac[NT][2], qsum[NT][2][NG];  // by this lane's columns 2 t, 2 t + 1 of the results
-      int seen[NT][2];
+  if (warp == NW) {
+    // -------------------------------------------------------------- loads: lane w for warp w
+    // A stage takes the next two records of a sequence and head (the last of them alone may
+    // be one): one copy where they lie in one page. Page numbers wait in shared memory, 64
+    // per warp: the lanes' own loads would each wait for the one before to return, since
+    // they write one register of the warp.
+    int x = ((int)blockIdx.x * NW + lane) * per;
+    const int end = lane < NW ? min(x + per, total) : x;
+    int entry = 0, in_page = 0, filled = 0, last = 0;  // page and record in it; pages read, the last one
+    auto enter = [&] {
+      entry = seg.at / a.page_tiles;
+      in_page = seg.at - entry * a.page_tiles;
+      last = (seg.nt - 1) / a.page_tiles;
+      filled = entry & ~31;
+    };
+    auto settle = [&] {  // to the next place that is a record
+      while (x < end && seg.at >= seg.nt) {
+        const int step = seg.stride - seg.at;
+        x += step;
+        if (x < end) advance(a, seg, step, same);
+      }
+      if (x < end) enter();
+    };
+    if (x < end) {
+      advance(a, seg, lane * per, same);
+      settle();
+    }
+    int put = 0;
+    uint32_t phase = 1, idle = 0;  // the first round finds the stages empty
+    uint64_t since = 0;
+    while (__any_sync(kFull, x < end)) {
+      for (uint32_t need; (need = __ballot_sync(kFull, x < end && filled <= min(entry + 8, last))) != 0u;) {
+        // 32 page numbers for each of these warps, four loads in flight
+        int got[4], who[4], base[4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int r = 8 * n + g;
-        float v[W][8];
-        float top = 0.f, sum[NG];
-#pragma unroll
-        for (int i = 0; i < NG; ++i) sum[i] = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const int gi = w / L::kGroupWords, j = w % L::kGroupWords;
-          uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-          if (r < rows)
-            raw = *reinterpret_cast<const uint4*>(
-                static_cast<const T*>(a.q) + seg.b * a.q_seq + ((row0 + r) / a.group) * a.q_token +
-                (int64_t)(kv_head * a.group + (row0 + r) % a.group) * a.q_head + gi * GS + t * (GS / 4) + 8 * j);
-          const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack2<T>(u[e]);
-            v[w][2 * e] = f.x;
-            v[w][2 * e + 1] = f.y;
-            sum[gi] += f.x + f.y;
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        }
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-        const float up = top > 0.f ? power_for(top, 13) : 1.0f;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          sum[i] += __shfl_xor_sync(kFull, sum[i], 1);
-          sum[i] += __shfl_xor_sync(kFull, sum[i], 2);
+        for (int k = 0; k < 4; ++k) {
+          who[k] = need ? __ffs(need) - 1 : -1;
+          need &= need - 1u;
+          const int w = max(who[k], 0);
+          base[k] = __shfl_sync(kFull, filled, w) + lane;
+          const int b = __shfl_sync(kFull, seg.b, w), to = __shfl_sync(kFull, last, w);
+          got[k] = who[k] >= 0 ? a.tables[b * a.table_stride + min(base[k], to)] : 0;
         }
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {  // two steps of 16 channels per word
-            qf[n][2 * w + k][0] = half2_bits(v[w][2 * k] * up, v[w][2 * k + 4] * up);
-            qf[n][2 * w + k][1] = half2_bits(v[w][2 * k + 1] * (up * 0.0625f), v[w][2 * k + 5] * (up * 0.0625f));
-          }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int src = 4 * (2 * t + c);
-          fac[n][c] = (1.0f / __shfl_sync(kFull, up, src)) * a.scale_log2 * 16777216.0f;
-#pragma unroll
-          for (int i = 0; i < NG; ++i) qsum[n][c][i] = __shfl_sync(kFull, sum[i], src) * a.scale_log2;
-          seen[n][c] = len - a.fresh + 1 + min((row0 + 8 * n + 2 * t + c) / a.group, a.fresh - 1);
+        for (int k = 0; k < 4; ++k) {
+          if (who[k] >= 0) s_pages[who[k]][base[k] & 63] = got[k];
+          if (lane == who[k]) filled += 32;
+        }
+        __syncwarp();
+      }
+      const bool go = x < end && mbar_test(&s_empty[lane][put], phase);
+      if (go) {
+        const bool both = min(seg.nt - seg.at, end - x) >= 2, whole = both && in_page + 1 < a.page_tiles;
+        const int page0 = s_pages[lane][entry & 63], page1 = s_pages[lane][(entry + 1) & 63];
+        const bool ok0 = page0 >= 0 && page0 < a.pages;
+        const bool ok1 = whole ? ok0 : both && page1 >= 0 && page1 < a.pages;
+        const int h = seg.h / a.parts;
+        const uint8_t* from =
+            a.cache + (((int64_t)page0 * a.kv_heads + h) * a.page_tiles + in_page) * L::kRecord;
+        unsigned char* to = smem + lane * P::kWarpRing + put * P::kStage;
+        uint64_t* bar = &s_full[lane][put];
+        s_gone[lane][put] = (ok0 ? 0u : 1u) | (ok1 ? 0u : 2u);
+        const uint32_t bytes = (ok0 ? L::kRecord : 0) + (ok1 ? L::kRecord : 0);
+        if (bytes > 0)
+          mbar_arrive_expect_tx(bar, bytes);
+        else
+          mbar_arrive(bar);
+        if (ok0) bulk_g2s(to, from, whole ? P::kStage : L::kRecord, bar);
+        if (ok1 && !whole)
+          bulk_g2s(to + L::kRecord, a.cache + ((int64_t)page1 * a.kv_heads + h) * a.page_tiles * L::kRecord, L::kRecord,
+                   bar);
+        const int n = both ? 2 : 1;
+        x += n;
+        seg.at += n;
+        in_page += n;
+        while (in_page >= a.page_tiles) {
+          in_page -= a.page_tiles;
+          ++entry;
+        }
+        if (seg.at >= seg.nt) settle();
+        if (++put == ST) {
+          put = 0;
+          phase ^= 1u;
         }
       }
-
-      float m[NT][2], ref[NT][2], l[NT][2], z[NT][2][NG];
-      float o[2 * W][NT][4];
-      // weights enter the product as p scale vf; back = 1 / vf, scales stay below the limit
-      float vf = 0x1p100f, back = 0x1p-100f, limit = (float)(2 << kTopScale) * back;
-      bool first = true;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          m[n][c] = -INFINITY;
-          ref[n][c] = 0.f;
-          l[n][c] = 0.f;
-#pragma unroll
-          for (int i = 0; i < NG; ++i) z[n][c][i] = 0.f;
+      if (__any_sync(kFull, go)) {
+        idle = 0;
+      } else {
+        __nanosleep(20);
+        if ((++idle & 4095u) == 1u) {  // bounded, like every wait
+          const uint64_t now = globaltimer_ns();
+          if (idle == 1u) since = now;
+          const bool late = now - since > kWaitNs || *reinterpret_cast<volatile unsigned*>(&g_wait_timeouts) != 0u;
+          if (__any_sync(kFull, late)) {
+            if (lane == 0) atomicAdd(&g_wait_timeouts, 1u);
+            break;
+          }
         }
-#pragma unroll
-        for (int k = 0; k < 2 * W; ++k)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[k][n][c] = 0.f;
       }
+    }
+  } else {
+    // -------------------------------------------------------------- a run, piece by piece
+    int x = ((int)blockIdx.x * NW + warp) * per;  // places x .. end
+    const int end = min(x + per, total);
+    if (x < end) advance(a, seg, warp * per, same);
+    unsigned char* ring = smem + warp * P::kWarpRing;
+    const uint32_t k_at = g * (D / 2) + t * (D / 8), p_at = g * (4 * NG),
+                   v_at = L::kV + t * D + (g ^ (2 * t)) * (4 * W);
+    int get = 0;
+    uint32_t phase = 0;
+    while (x < end) {
+      const int t0 = seg.at, t1 = min(seg.nt, seg.at + (end - x));  // this piece's records
+      if (t0 < t1) {
+        const int kv_head = seg.h / a.parts, row0 = (seg.h - kv_head * a.parts) * P::kRows;
+        const int rows = min(a.fresh * a.group - row0, P::kRows);
+        const int len = min(max(a.lens[seg.b], 0), a.max_len);
+        const int see = len - a.fresh + 1 + (a.fresh == 1 ? 0 : row0 / a.group);  // tokens that the first row sees
 
-      // The two records at `rec`, the first of them number `tile`; masked: some row does not
-      // see some token, or there is only one record (bits of `gone`: not there).
-      auto consume = [&](auto masked_type, const uint8_t* rec, int tile, uint32_t gone) {
-        constexpr bool kMasked = decltype(masked_type)::value;
-        // scores: tokens g and g + 8 of a record, columns 2 t and 2 t + 1
-        float s[2][NT][4];
-        uint32_t ka[2][W], kb[2][W], pa[2][NG], pb[2][NG];
+        // q as operand B: column g of block n is query row 8 n + g; this lane's channels are
+        // those of chunk t of a K row. f16 with the row's largest value near 2^13, so that the
+        // half of them that is divided by 16 keeps its bits; below 2^-22 of the largest they
+        // are rounded, which moves no score by more than 2^-24 of its largest term.
+        const T* q = static_cast<const T*>(a.q) + seg.b * a.q_seq + t * (GS / 4);
+        uint32_t raw[NT][W][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint8_t* k = rec + i * L::kRecord;
-          load_words(k + g * (D / 2) + t * (D / 8), ka[i]);
-          load_words(k + (g + 8) * (D / 2) + t * (D / 8), kb[i]);
-          load_words(k + L::kKParams + g * (4 * NG), pa[i]);
-          load_words(k + L::kKParams + (g + 8) * (4 * NG), pb[i]);
-        }
+        for (int n = 0; n < NT; ++n) {
+          const int r = row0 + 8 * n + g;
+          const int j = a.fresh == 1 ? 0 : r / a.group;
+          const T* from = q + j * a.q_token + (int64_t)(kv_head * a.group + r - j * a.group) * a.q_head;
 #pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          float acc[2][NT][4];
-#pragma unroll
-          for (int j = 0; j < L::kGroupWords; ++j) {
-            const int w = gi * L::kGroupWords + j;
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t u = ka[i][w] >> (8 * q), v = kb[i][w] >> (8 * q);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  if (j == 0 && q == 0)
-                    mma_m16n8k16_zero(acc[i][n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
-                                      qf[n][2 * w + q][0], qf[n][2 * w + q][1]);
-                  else
-                    mma_m16n8k16(acc[i][n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
-                                 qf[n][2 * w + q][0], qf[n][2 * w + q][1]);
-                }
-              }
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float2 qa = unpack2<T>(pa[i][gi]), qb = unpack2<T>(pb[i][gi]);  // scale, zero
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const float za = gi == 0 ? qa.y * qsum[n][c][gi] : fmaf(qa.y, qsum[n][c][gi], s[i][n][c]);
-                const float zb = gi == 0 ? qb.y * qsum[n][c][gi] : fmaf(qb.y, qsum[n][c][gi], s[i][n][2 + c]);
-                s[i][n][c] = fmaf(qa.x * acc[i][n][c], fac[n][c], za);
-                s[i][n][2 + c] = fmaf(qb.x * acc[i][n][2 + c], fac[n][c], zb);
-              }
+          for (int w = 0; w < W; ++w) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (8 * n + g < rows)
+              v = *reinterpret_cast<const uint4*>(from + w / L::kGroupWords * GS + w % L::kGroupWords * 8);
+            raw[n][w][0] = v.x, raw[n][w][1] = v.y, raw[n][w][2] = v.z, raw[n][w][3] = v.w;
           }
         }
-        if constexpr (kMasked) {
+        uint32_t qf[NT][D / 16][2];
+        float fac[NT][2], qsum[NT][2][NG];  // by this lane's columns 2 t, 2 t + 1 of the results
+        int seen[NT][2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int at = (tile + i) * kTile + g;
-            const bool none = (gone >> i) & 1u;
+        for (int n = 0; n < NT; ++n) {
+          const T2 zero2 = two<T>(0u);
+          T2 most = zero2;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+          for (int w = 0; w < W; ++w)
 #pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                if (none || at >= seen[n][c]) s[i][n][c] = -INFINITY;
-                if (none || at + 8 >= seen[n][c]) s[i][n][2 + c] = -INFINITY;
-              }
-          }
-        }
-        // V's scales and zeros of the lane's tokens
-        float sv[2][2][NG], zv[2][2][NG];
-        float wide = 0.f;
+            for (int e = 0; e < 4; ++e) most = __hmax2(most, __habs2(two<T>(raw[n][w][e])));
+          float top = fmaxf(Act<T>::to_f(most.x), Act<T>::to_f(most.y));
+          top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+          const float up = top > 0.f ? power_for(top, 13) : 1.0f;
+          float sum[NG];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          load_words(rec + i * L::kRecord + L::kVParams + g * (4 * NG), pa[i]);
-          load_words(rec + i * L::kRecord + L::kVParams + (g + 8) * (4 * NG), pb[i]);
+          for (int i = 0; i < NG; ++i) sum[i] = 0.f;
 #pragma unroll
-          for (int k = 0; k < NG; ++k) {
-            const float2 u = unpack2<T>(pa[i][k]), v = unpack2<T>(pb[i][k]);
-            sv[i][0][k] = u.x, zv[i][0][k] = u.y, sv[i][1][k] = v.x, zv[i][1][k] = v.y;
-            if constexpr (kMasked) {  // what lies behind the sequence may be anything
-              const int at = (tile + i) * kTile + g;
-              const bool none = (gone >> i) & 1u;
-              if (none || at >= len) sv[i][0][k] = zv[i][0][k] = 0.f;
-              if (none || at + 8 >= len) sv[i][1][k] = zv[i][1][k] = 0.f;
+          for (int w = 0; w < W; ++w) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = unpack2<T>(raw[n][w][e]);
+              v[2 * e] = f.x, v[2 * e + 1] = f.y;
+              sum[w / L::kGroupWords] += f.x + f.y;
             }
-            wide = fmaxf(wide, fmaxf(sv[i][0][k], sv[i][1][k]));
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // two steps of 16 channels per word
+              qf[n][2 * w + k][0] = half2_bits(v[2 * k] * up, v[2 * k + 4] * up);
+              qf[n][2 * w + k][1] = half2_bits(v[2 * k + 1] * (up * 0.0625f), v[2 * k + 5] * (up * 0.0625f));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            sum[i] += __shfl_xor_sync(kFull, sum[i], 1);
+            sum[i] += __shfl_xor_sync(kFull, sum[i], 2);
+          }
+          // 1 / up, and 2^24 for the codes' subnormals, by the exponent
+          const float down = __uint_as_float((278u << 23) - __float_as_uint(up));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int src = 4 * (2 * t + c), r = row0 + 8 * n + 2 * t + c;
+            fac[n][c] = __shfl_sync(kFull, down, src) * a.scale_log2;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) qsum[n][c][i] = __shfl_sync(kFull, sum[i], src) * a.scale_log2;
+            seen[n][c] = len - a.fresh + 1 + (a.fresh == 1 ? 0 : min(r / a.group, a.fresh - 1));
           }
         }
-        // Weights by the maximum so far. Where they sum to more than kSlack the maximum is
-        // raised and they are made anew; `first` makes that so until every row has a maximum.
-        float p[2][NT][4], add[NT][2];
-        auto weigh = [&] {
+
+        float m[NT][2], ref[NT][2], l[NT][2], z[NT][2][NG];
+        float o[2 * W][NT][4];
+        // weights enter the product as p scale vf; back = 1 / vf, scales stay below the limit
+        float vf = 0x1p100f, back = 0x1p-100f, limit = (float)(2 << kTopScale) * back;
+        bool first = true;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            m[n][c] = -INFINITY;
+            ref[n][c] = 0.f;
+            l[n][c] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) z[n][c][i] = 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < 2 * W; ++k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[k][n][c] = 0.f;
+        }
+
+        const int clear = min(t1, see / kTile);  // records before this one are seen whole by all rows
+#pragma unroll 1
+        for (int tile = t0; tile < t1; tile += 2) {
+          mbar_wait_nocall(&s_full[warp][get], phase);
+          const unsigned char* rec = ring + get * P::kStage;
+          const uint32_t gone = s_gone[warp][get];
+          const bool masked = tile + 2 > clear || gone != 0u;  // a row does not see a token, or there is none
+          // scores: tokens g and g + 8 of a record, columns 2 t and 2 t + 1
+          float s[2][NT][4];
+          uint32_t ka[2][W], kb[2][W], pa[2][NG], pb[2][NG];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            load_words(rec + i * L::kRecord + k_at, ka[i]);
+            load_words(rec + i * L::kRecord + 4 * D + k_at, kb[i]);
+            load_words(rec + i * L::kRecord + L::kKParams + p_at, pa[i]);
+            load_words(rec + i * L::kRecord + L::kKParams + 32 * NG + p_at, pb[i]);
+          }
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            float acc[2][NT][4];
+#pragma unroll
+            for (int j = 0; j < L::kGroupWords; ++j) {
+              const int w = gi * L::kGroupWords + j;
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const uint32_t u = ka[i][w] >> (8 * q), v = kb[i][w] >> (8 * q);
+#pragma unroll
+                  for (int n = 0; n < NT; ++n) {
+                    if (j == 0 && q == 0)
+                      mma_m16n8k16_zero(acc[i][n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
+                                        qf[n][2 * w + q][0], qf[n][2 * w + q][1]);
+                    else
+                      mma_m16n8k16(acc[i][n], u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u,
+                                   qf[n][2 * w + q][0], qf[n][2 * w + q][1]);
+                  }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 qa = unpack2<T>(pa[i][gi]), qb = unpack2<T>(pb[i][gi]);  // scale, zero
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  const float za = gi == 0 ? qa.y * qsum[n][c][gi] : fmaf(qa.y, qsum[n][c][gi], s[i][n][c]);
+                  const float zb = gi == 0 ? qb.y * qsum[n][c][gi] : fmaf(qb.y, qsum[n][c][gi], s[i][n][2 + c]);
+                  s[i][n][c] = fmaf(qa.x * acc[i][n][c], fac[n][c], za);
+                  s[i][n][2 + c] = fmaf(qb.x * acc[i][n][2 + c], fac[n][c], zb);
+                }
+            }
+          }
+          // V's scales and zeros of the lane's tokens
+          float sv[2][2][NG], zv[2][2][NG];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            load_words(rec + i * L::kRecord + L::kVParams + p_at, pa[i]);
+            load_words(rec + i * L::kRecord + L::kVParams + 32 * NG + p_at, pb[i]);
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+              const float2 u = unpack2<T>(pa[i][k]), v = unpack2<T>(pb[i][k]);
+              sv[i][0][k] = u.x, zv[i][0][k] = u.y, sv[i][1][k] = v.x, zv[i][1][k] = v.y;
+            }
+          }
+          if (masked) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) p[i][n][c] = exp2_fast(s[i][n][c] - ref[n][c & 1]);
+              for (int b = 0; b < 2; ++b) {
+                const int at = (gone >> i) & 1u ? 0x7fffffff : (tile + i) * kTile + g + 8 * b;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) add[n][c] = (p[0][n][c] + p[0][n][2 + c]) + (p[1][n][c] + p[1][n][2 + c]);
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                  for (int c = 0; c < 2; ++c)
+                    if (at >= seen[n][c]) s[i][n][2 * b + c] = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < NG; ++k)  // what lies behind the sequence may be anything
+                  if (at >= len) sv[i][b][k] = zv[i][b][k] = 0.f;
+              }
           }
-        };
-        weigh();
-        bool grow = first || wide > limit;
+          float wide = 0.f;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) grow = grow || fmaxf(add[n][0], add[n][1]) > kSlack;
-        if (__any_sync(kFull, grow)) {
-          bool unset = false;
+          for (int k = 0; k < NG; ++k)
+            wide = fmaxf(fmaxf(wide, fmaxf(sv[0][0][k], sv[0][1][k])), fmaxf(sv[1][0][k], sv[1][1][k]));
+          // Weights by the maximum so far. Where they sum to more than kSlack the maximum is
+          // raised and they are made anew; `first` makes that so until every row has a maximum.
+          float p[2][NT][4], add[NT][2];
+#pragma unroll 1
+          for (bool raised = false;; raised = true) {
+            bool grow = first || wide > limit;
 #pragma unroll
-          for (int k = 4; k < 32; k *= 2) wide = fmaxf(wide, __shfl_xor_sync(kFull, wide, k));
-          float turn = 1.0f;
-          if (wide > limit) {
-            const float now = power_for(wide, kTopScale);
-            turn = now * back;
-            vf = now;
-            back = 1.0f / now;
-            limit = (float)(2 << kTopScale) * back;
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) p[i][n][c] = exp2_fast(s[i][n][c] - ref[n][c & 1]);
+#pragma unroll
+              for (int c = 0; c < 2; ++c) add[n][c] = (p[0][n][c] + p[0][n][2 + c]) + (p[1][n][c] + p[1][n][2 + c]);
+              grow = grow || fmaxf(add[n][0], add[n][1]) > kSlack;
+            }
+            if (raised || !__any_sync(kFull, grow)) break;
+#pragma unroll
+            for (int k = 4; k < 32; k *= 2) wide = fmaxf(wide, __shfl_xor_sync(kFull, wide, k));
+            float turn = 1.0f;
+            if (wide > limit) {
+              const float now = power_for(wide, kTopScale);
+              turn = now * back;
+              vf = now;
+              back = 1.0f / now;
+              limit = (float)(2 << kTopScale) * back;
+            }
+            bool unset = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                float top = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
+#pragma unroll
+                for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, k));
+                float f = 1.0f;
+                if (top > m[n][c]) {
+                  f = exp2_fast(m[n][c] - top);
+                  m[n][c] = ref[n][c] = top;
+                }
+                unset = unset || m[n][c] == -INFINITY;
+                l[n][c] *= f;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) z[n][c][i] *= f;
+#pragma unroll
+                for (int k = 0; k < 2 * W; ++k) {
+                  o[k][n][c] *= f * turn;
+                  o[k][n][2 + c] *= f * turn;
+                }
+              }
+            first = __any_sync(kFull, unset);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float top = fmaxf(fmaxf(s[0][n][c], s[0][n][2 + c]), fmaxf(s[1][n][c], s[1][n][2 + c]));
+            for (int c = 0; c < 2; ++c) l[n][c] += add[n][c];
 #pragma unroll
-              for (int k = 4; k < 32; k *= 2) top = fmaxf(top, __shfl_xor_sync(kFull, top, k));
-              float f = 1.0f;
-              if (top > m[n][c]) {
-                f = exp2_fast(m[n][c] - top);
-                m[n][c] = ref[n][c] = top;
-              }
-              unset = unset || m[n][c] == -INFINITY;
-              l[n][c] *= f;
+          for (int i = 0; i < 2; ++i) {
+            uint32_t va[W], vb[W];
+            load_words(rec + i * L::kRecord + v_at, va);
+            load_words(rec + i * L::kRecord + 4 * D + v_at, vb);
+            // weights x scale as operand B of the output's product
+            uint32_t pf[NT][NG][2];
 #pragma unroll
-              for (int i = 0; i < NG; ++i) z[n][c][i] *= f;
+            for (int n = 0; n < NT; ++n) {
+              const float* w = p[i][n];
 #pragma unroll
-              for (int k = 0; k < 2 * W; ++k) {
-                o[k][n][c] *= f * turn;
-                o[k][n][2 + c] *= f * turn;
+              for (int k = 0; k < NG; ++k) {
+                const float sa = sv[i][0][k] * vf, sb = sv[i][1][k] * vf;
+                float u[4] = {w[0] * sa, w[1] * sa, w[2] * sb, w[3] * sb};
+                float y[4] = {w[0] * zv[i][0][k], w[1] * zv[i][0][k], w[2] * zv[i][1][k], w[3] * zv[i][1][k]};
+                if (masked) {  // a token that this row does not see may hold NaN
+#pragma unroll
+                  for (int c = 0; c < 4; ++c)
+                    if (s[i][n][c] == -INFINITY) u[c] = y[c] = 0.f;
+                }
+                const uint32_t ha = half2_bits(u[0], u[1]), hb = half2_bits(u[2], u[3]);
+                z[n][0][k] += y[0] + y[2];
+                z[n][1][k] += y[1] + y[3];
+                if constexpr (!Act<T>::kBf16) {
+                  // What the 11 bits lose is given back for a code of 7.5, the middle of the
+                  // range, so that the error left is that of v's spread and not of its offset:
+                  // fp16 outputs would show it (3.5e-4 relative without, 2.4e-4 with), bf16's
+                  // own rounding (1.7e-3) hides it.
+                  const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&ha));
+                  const float2 rb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
+                  z[n][0][k] = fmaf((u[0] - ra.x) + (u[2] - rb.x), 7.5f * back, z[n][0][k]);
+                  z[n][1][k] = fmaf((u[1] - ra.y) + (u[3] - rb.y), 7.5f * back, z[n][1][k]);
+                }
+                pf[n][k][0] = transpose_8x8(ha);
+                pf[n][k][1] = transpose_8x8(hb);
               }
             }
-          first = __any_sync(kFull, unset);
-          weigh();
+            // Rows g are fed the whole byte 16 hi + lo, rows g + 8 its 16 hi: their difference
+            // in the end is lo's sum, exact but for fp32's rounding, and an AND fewer per word.
+#pragma unroll
+            for (int w = 0; w < W; ++w)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const uint32_t u = k == 0 ? va[w] & 0x00ff00ffu : __byte_perm(va[w], 0u, 0x4341u);
+                const uint32_t y = k == 0 ? vb[w] & 0x00ff00ffu : __byte_perm(vb[w], 0u, 0x4341u);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                  mma_m16n8k16(o[2 * w + k][n], u, u & 0x00f000f0u, y, y & 0x00f000f0u, pf[n][w / L::kGroupWords][0],
+                               pf[n][w / L::kGroupWords][1]);
+              }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[warp][get]);
+          if (++get == ST) {
+            get = 0;
+            phase ^= 1u;
+          }
         }
+
+        // ---------------------------------------------------------- the piece's sums
+        const bool began = t0 > 0, goes = t1 < seg.nt;
+        // the run's last piece leaves its sums where the ring was
+        const bool last = x + (t1 - t0) >= end || (x + (seg.stride - seg.at) >= end);
+        float* sums = last ? reinterpret_cast<float*>(ring) : heads_of + warp * P::kSums;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) l[n][c] += add[n][c];
+          for (int c = 0; c < 2; ++c) {
+            const int r = 8 * n + 2 * t + c;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          // weights x scale as operand B of the output's product
-          uint32_t pf[NT][NG][2];
+            for (int k = 4; k < 32; k *= 2) {
+              l[n][c] += __shfl_xor_sync(kFull, l[n][c], k);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float* w = p[i][n];
+              for (int i = 0; i < NG; ++i) z[n][c][i] += __shfl_xor_sync(kFull, z[n][c][i], k);
+            }
+            if ((began || goes) && g == 0) {
+              sums[P::kRows * P::kRow + r] = m[n][c];
+              sums[P::kRows * P::kRow + P::kRows + r] = l[n][c];
+            }
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
-              const float sa = sv[i][0][k] * vf, sb = sv[i][1][k] * vf;
-              float u[4] = {w[0] * sa, w[1] * sa, w[2] * sb, w[3] * sb};
-              float zp[4] = {zv[i][0][k], zv[i][0][k], zv[i][1][k], zv[i][1][k]};
-              if constexpr (kMasked) {  // a token that this row does not see may hold NaN
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                  if (s[i][n][c] == -INFINITY) u[c] = zp[c] = 0.f;
+            for (int w = 0; w < W; ++w) {
+              const int gi = w / L::kGroupWords, j = w % L::kGroupWords;
+              const int d = gi * GS + g * (GS / 8) + 4 * j;
+              const float f = back * 16777216.0f;
+              const float4 v = make_float4(fmaf(o[2 * w][n][c] - o[2 * w][n][2 + c], f, z[n][c][gi]),
+                                           fmaf(o[2 * w][n][2 + c], f * 0.0625f, z[n][c][gi]),
+                                           fmaf(o[2 * w + 1][n][c] - o[2 * w + 1][n][2 + c], f, z[n][c][gi]),
+                                           fmaf(o[2 * w + 1][n][2 + c], f * 0.0625f, z[n][c][gi]));
+              if (began || goes) {
+                *reinterpret_cast<float4*>(sums + r * P::kRow + d) = v;
+              } else if (r < rows) {
+                finish(seg.b, kv_head, row0 + r, d, m[n][c], l[n][c], v);
               }
-              const uint32_t ha = half2_bits(u[0], u[1]), hb = half2_bits(u[2], u[3]);
-              z[n][0][k] = fmaf(w[0], zp[0], fmaf(w[2], zp[2], z[n][0][k]));
-              z[n][1][k] = fmaf(w[1], zp[1], fmaf(w[3], zp[3], z[n][1][k]));
-              if constexpr (!Act<T>::kBf16) {
-                // What the 11 bits lose is given back for a code of 7.5, the middle of the
-                // range, so that the error left is that of v's spread and not of its offset:
-                // fp16 outputs would show it (3.5e-4 relative without, 2.4e-4 with), bf16's
-                // own rounding (1.7e-3) hides it.
-                const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&ha));
-                const float2 rb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
-                z[n][0][k] = fmaf((u[0] - ra.x) + (u[2] - rb.x), 7.5f * back, z[n][0][k]);
-                z[n][1][k] = fmaf((u[1] - ra.y) + (u[3] - rb.y), 7.5f * back, z[n][1][k]);
-              }
-              pf[n][k][0] = transpose_8x8(ha);
-              pf[n][k][1] = transpose_8x8(hb);
             }
           }
-          uint32_t va[W], vb[W];
-          const uint8_t* v = rec + i * L::kRecord + L::kV + t * D + ((g ^ (2 * t)) * W) * 4;
-          load_words(v, va);
-          load_words(v + 4 * D, vb);
-          // Rows g are fed the whole byte 16 hi + lo, rows g + 8 its 16 hi: their difference
-          // in the end is lo's sum, exact but for fp32's rounding, and an AND fewer per word.
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t u = k == 0 ? va[w] & 0x00ff00ffu : __byte_perm(va[w], 0u, 0x4341u);
-              const uint32_t y = k == 0 ? vb[w] & 0x00ff00ffu : __byte_perm(vb[w], 0u, 0x4341u);
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-                mma_m16n8k16(o[2 * w + k][n], u, u & 0x00f000f0u, y, y & 0x00f000f0u, pf[n][w / L::kGroupWords][0],
-                             pf[n][w / L::kGroupWords][1]);
-            }
-        }
-      };
-      const int clear = min(t1, see / kTile);  // records before this one are seen whole by all rows
-      auto release = [&] {
-        __syncwarp();
-        load(get);
-        if (++get == ST) {
-          get = 0;
-          phase ^= 1;
-        }
-      };
-      // a loop of its own for the records that need no mask: a choice in each step would
-      // have the sums moved between registers (28 % more instructions)
-      for (int tile = t0; tile < t1;) {
-#pragma unroll 1
-        for (; tile + 2 <= clear && ((bad >> (2 * get)) & 3u) == 0; tile += 2) {
-          mbar_wait_nocall(&bars[get], phase);
-          consume(std::false_type{}, ring + get * P::kStage, tile, 0u);
-          release();
-        }
-        if (tile >= t1) break;
-        const uint32_t gone = (bad >> (2 * get)) & 3u;
-        mbar_wait_nocall(&bars[get], phase);
-        consume(std::true_type{}, ring + get * P::kStage, tile, tile + 1 < t1 ? gone : gone | 2u);
-        release();
-        tile += 2;
-      }
-
-      // ---------------------------------------------------------- the piece's sums
-      const bool began = t0 > 0, goes = t1 < seg.nt;
-      float* sums = began ? s_sums + warp * P::kSums : reinterpret_cast<float*>(ring);
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int r = 8 * n + 2 * t + c;
-#pragma unroll
-          for (int k = 4; k < 32; k *= 2) {
-            l[n][c] += __shfl_xor_sync(kFull, l[n][c], k);
-#pragma unroll
-            for (int i = 0; i < NG; ++i) z[n][c][i] += __shfl_xor_sync(kFull, z[n][c][i], k);
+        if (lane == 0 && (began || goes)) {
+          const Piece piece{seg.b, seg.h, x - seg.at, seg.nt};
+          if (began) {
+            s_left[warp].flags |= (goes ? kHead | kThrough : kHead) | (last ? 0 : kAway);
+            s_left[warp].head = piece;
+          } else {
+            s_left[warp].flags |= kTail;
+            s_left[warp].tail = piece;
           }
-          if ((began || goes) && g == 0) {
-            sums[P::kRows * P::kRow + r] = m[n][c];
-            sums[P::kRows * P::kRow + P::kRows + r] = l[n][c];
-          }
-#pragma unroll
-          for (int w = 0; w < W; ++w) {
-            const int gi = w / L::kGroupWords, j = w % L::kGroupWords;
-            const int d = gi * GS + g * (GS / 8) + 4 * j;
-            const float f = back * 16777216.0f;
-            const float4 v = make_float4(fmaf(o[2 * w][n][c] - o[2 * w][n][2 + c], f, z[n][c][gi]),
-                                         fmaf(o[2 * w][n][2 + c], f * 0.0625f, z[n][c][gi]),
-                                         fmaf(o[2 * w + 1][n][c] - o[2 * w + 1][n][2 + c], f, z[n][c][gi]),
-                                         fmaf(o[2 * w + 1][n][2 + c], f * 0.0625f, z[n][c][gi]));
-            if (began || goes) {
-              *reinterpret_cast<float4*>(sums + r * P::kRow + d) = v;
-            } else if (r < rows) {
-              finish(seg.b, kv_head, row0 + r, d, m[n][c], l[n][c], v);
-            }
-          }
-        }
-      if (lane == 0 && (began || goes)) {
-        const Piece piece{seg.b, seg.h, x - seg.at, seg.nt};
-        if (began) {
-          s_left[warp].flags |= goes ? kHead | kThrough : kHead;
-          s_left[warp].head = piece;
-        } else {
-          s_left[warp].flags |= kTail;
-          s_left[warp].tail = piece;
         }
       }
+      const int step = min(seg.stride - seg.at, end - x);
+      x += step;
+      if (x < end) advance(a, seg, step, same);
     }
-    const int step = min(seg.stride - seg.at, end - x);
-    x += step;
-    if (x < end) advance(a, seg, step, same);
   }
 
   // ---------------------------------------------------------------- join what warps share
@@ -717,38 +756,35 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
   // leaves open; a chain takes the heads of the warps behind it while they go through.
   // A thread takes 4 channels of a row of a chain.
   const int all = a.fresh * a.group;
-  constexpr int kItems = P::kRows * (D / 4);
-  for (int i = threadIdx.x; i < (NW + 1) * kItems; i += P::kThreads) {
-    const int chain = i / kItems, r = i % kItems / (D / 4), d = 4 * (i % (D / 4));
+#pragma unroll 1
+  for (int chain = 0; chain <= NW; ++chain) {
     const Left& first = s_left[max(chain - 1, 0)];
     if (!(first.flags & (chain == 0 ? kHead : kTail))) continue;
     const Piece piece = chain == 0 ? first.head : first.tail;
-    const int kv_head = piece.h / a.parts, row = (piece.h - kv_head * a.parts) * P::kRows + r;
-    if (row >= all) continue;
-    int w1 = max(chain - 1, 0);  // the chain's last warp
+    const int kv_head = piece.h / a.parts, row0 = (piece.h - kv_head * a.parts) * P::kRows;
+    const int w0 = max(chain - 1, 0);
+    int w1 = w0;  // the chain's last warp
     bool open = chain > 0 || (first.flags & kThrough);
     while (open && w1 + 1 < NW) open = s_left[++w1].flags & kThrough;
-    auto part = [&](int w) {
-      return w == chain - 1 ? reinterpret_cast<const float*>(smem + w * P::kWarpRing) : s_sums + w * P::kSums;
-    };
-    float top = -INFINITY, sum = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = max(chain - 1, 0); w <= w1; ++w) top = fmaxf(top, part(w)[P::kRows * P::kRow + r]);
-    for (int w = max(chain - 1, 0); w <= w1; ++w) {
-      const float* from = part(w);
-      const float lw = from[P::kRows * P::kRow + P::kRows + r];
-      if (lw == 0.f) continue;  // this warp saw nothing (a NaN sum counts)
-      const float f = exp2_fast(from[P::kRows * P::kRow + r] - top);
-      const float4 y = *reinterpret_cast<const float4*>(from + r * P::kRow + d);
-      sum = fmaf(lw, f, sum);
-      v.x = fmaf(y.x, f, v.x), v.y = fmaf(y.y, f, v.y), v.z = fmaf(y.z, f, v.z), v.w = fmaf(y.w, f, v.w);
-    }
-    if (chain > 0 && !open) {
-      finish(piece.b, kv_head, row, d, top, sum, v);
-    } else {
-      float* slot = a.slots + ((int64_t)blockIdx.x * 2 + (chain > 0)) * P::kRows * (D + 2);
-      __stcg(reinterpret_cast<float4*>(slot + 2 * P::kRows + r * D + d), v);
-      if (d == 0) __stcg(reinterpret_cast<float2*>(slot + 2 * r), make_float2(top, sum));
+    for (int i = threadIdx.x; i < min(all - row0, P::kRows) * (D / 4); i += P::kThreads) {
+      const int r = i / (D / 4), d = 4 * (i % (D / 4));
+      float top = -INFINITY, sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int w = w0; w <= w1; ++w) {
+        const bool away = w >= chain && (s_left[w].flags & kAway);
+        const float* from =
+            away ? heads_of + w * P::kSums : reinterpret_cast<const float*>(smem + w * P::kWarpRing);
+        add_sums(top, sum, v, from[P::kRows * P::kRow + r], from[P::kRows * P::kRow + P::kRows + r],
+                 *reinterpret_cast<const float4*>(from + r * P::kRow + d));
+      }
+      if (chain > 0 && !open) {
+        finish(piece.b, kv_head, row0 + r, d, top, sum, v);
+      } else {
+        float* slot = a.slots + ((int64_t)blockIdx.x * 2 + (chain > 0)) * P::kRows * (D + 2);
+        __stcg(reinterpret_cast<float4*>(slot + 2 * P::kRows + r * D + d), v);
+        if (d == 0) __stcg(reinterpret_cast<float2*>(slot + 2 * r), make_float2(top, sum));
+      }
     }
   }
   // The sequences and heads that other CTAs share: the one that came from the CTA before,
@@ -763,14 +799,14 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
   }
   const bool before = s_left[0].flags & kHead;
   if (!before && !after) return;
-  __threadfence();
-  __syncthreads();
+  __syncthreads();  // the slots are written; the fence below covers them for the whole CTA
   if (threadIdx.x < 2) {
     const bool mine = threadIdx.x == 0 ? before : after;
     bool last = false;
     if (mine) {
       const Piece p = threadIdx.x == 0 ? s_left[0].head : s_left[from].tail;
       const int c0 = p.first / per / NW, c1 = (p.first + p.nt - 1) / per / NW;
+      __threadfence();
       last = atomicAdd(&a.tickets[c0], 1u) == (unsigned)(c1 - c0);
       if (last) a.tickets[c0] = 0u;  // ready for the next launch
       __threadfence();
@@ -786,17 +822,22 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, Plan<D, GS, NT>::kC
     const int kv_head = p.h / a.parts, row0 = (p.h - kv_head * a.parts) * P::kRows;
     for (int i = threadIdx.x; i < min(all - row0, P::kRows) * (D / 4); i += P::kThreads) {
       const int r = i / (D / 4), d = 4 * (i % (D / 4));
-      auto part = [&](int c) { return a.slots + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * P::kRows * (D + 2); };
+      // the slots of four CTAs at a time, for the loads' latency
       float top = -INFINITY, sum = 0.f;
-      for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part(c) + 2 * r));
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int c = c0; c <= c1; ++c) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part(c) + 2 * r));
-        if (ml.y == 0.f) continue;
-        const float f = exp2_fast(ml.x - top);
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(part(c) + 2 * P::kRows + r * D + d));
-        sum = fmaf(ml.y, f, sum);
-        v.x = fmaf(y.x, f, v.x), v.y = fmaf(y.y, f, v.y), v.z = fmaf(y.z, f, v.z), v.w = fmaf(y.w, f, v.w);
+      for (int c = c0; c <= c1; c += 4) {
+        float2 ml[4];
+        float4 y[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float* from = a.slots + ((int64_t)min(c + k, c1) * 2 + (c + k == c0 ? 1 : 0)) * P::kRows * (D + 2);
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(from + 2 * r));
+          y[k] = __ldcg(reinterpret_cast<const float4*>(from + 2 * P::kRows + r * D + d));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (c + k <= c1) add_sums(top, sum, v, ml[k].x, ml[k].y, y[k]);
+        }
       }
       finish(p.b, kv_head, row0 + r, d, top, sum, v);
     }
@@ -814,7 +855,7 @@ int sm_count() {
 }
 
 constexpr size_t kTicketRegion = 16 << 10;  // where the linears keep theirs: all zero between calls
-static_assert(kTicketRegion >= 4 * kMaxCtas * 1024, "a ticket per CTA");
+static_assert(kTicketRegion >= 4 * 1024, "a ticket per CTA, one CTA per SM");
 
 int row_tiles(int64_t rows) { return rows <= 8 ? 1 : 2; }  // blocks of 8 query rows of a warp
 
@@ -824,7 +865,7 @@ int launch(const Kv4AttnArgs& a, int sms, cudaStream_t st) {
   auto kern = kv4_attention_kernel<T, D, GS, NT>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmem);
   if (e != cudaSuccess) return set_error(GRINQH_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  kern<<<(unsigned)(P::kCtas * sms), P::kThreads, P::kSmem, st>>>(a);
+  kern<<<(unsigned)sms, P::kThreads, P::kSmem, st>>>(a);
   return check_launch("kv4_attention");
 }
 
@@ -843,9 +884,10 @@ using namespace grinqh;
 
 extern "C" size_t grinqh_kv4_attention_workspace_size(int64_t num_seqs, int new_tokens, int num_heads,
                                                       int num_kv_heads, int head_dim) {
-  if (num_seqs <= 0 || num_kv_heads <= 0) return 0;
+  if (num_seqs <= 0 || new_tokens <= 0 || num_kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
   const int rows = 8 * row_tiles((int64_t)new_tokens * (num_heads / num_kv_heads));
-  return kTicketRegion + (size_t)kMaxCtas * sm_count() * 2 * rows * (head_dim + 2) * sizeof(float);
+  const size_t warps = rows == 16 && head_dim == 128 ? 7 : 15;
+  return kTicketRegion + (size_t)sm_count() * (2 * rows * (head_dim + 2) + warps * rows * (head_dim + 6)) * sizeof(float);
 }
 
 extern "C" int grinqh_kv4_attention(const void* q, int dtype, int64_t num_seqs, int new_tokens, int num_heads,
@@ -892,7 +934,9 @@ extern "C" int grinqh_kv4_attention(const void* q, int dtype, int64_t num_seqs, 
   a.out = out;
   a.lse = lse;
   a.tickets = static_cast<unsigned*>(workspace);
+  const int tiles = row_tiles((int64_t)new_tokens * (num_heads / num_kv_heads));
   a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kTicketRegion);
+  a.sums = a.slots + (size_t)sms * 2 * 8 * tiles * (head_dim + 2);
   a.table_stride = table_stride;
   a.pages = num_pages;
   a.seqs = (int)num_seqs;
@@ -904,10 +948,9 @@ extern "C" int grinqh_kv4_attention(const void* q, int dtype, int64_t num_seqs, 
   a.max_len = (int)(table_width * page_size);
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   if (!(flags & GRINQH_WORKSPACE_ZEROED)) {
-    const cudaError_t e = cudaMemsetAsync(workspace, 0, (size_t)kMaxCtas * sms * sizeof(unsigned), stream);
+    const cudaError_t e = cudaMemsetAsync(workspace, 0, (size_t)sms * sizeof(unsigned), stream);
     if (e != cudaSuccess) return set_error(GRINQH_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
   }
-  const int tiles = row_tiles((int64_t)new_tokens * a.group);
   a.parts = (new_tokens * a.group + 8 * tiles - 1) / (8 * tiles);
   return kv4_dispatch(head_dim, group_size, [&](auto layout) {
     using L = decltype(layout);
