@@ -7,11 +7,14 @@
 // maximum exceeds it by less than kSlack: the weights then reach at most 2^kSlack, no
 // accumulator is rescaled, and the division by l in the end makes up for it.
 //
-// A CTA computes two tiles of 128 queries at once, so that one tile's softmax runs while
-// the tensor cores work on the other's: two heads of one kv head over the same rows where
-// the group is even (they share K and V and see the same keys), else two row tiles of one
-// head.
-//   warp 8     loads Q once and blocks of 128 keys of K and V through a ring, by TMA
+// A tile is 128 rows: as many tokens as its query heads of one kv head allow, token by
+// token (which a TMA box of {64 channels, heads, tokens} lays out by itself), so a short
+// prompt fills its tiles with all heads that share K and V. An item is two tiles, so that
+// one tile's softmax runs while the tensor cores work on the other's. The grid has a CTA
+// per item, those that see the most keys first; the CTA that an SM runs takes over the
+// items of CTAs that have not started (cluster launch control) and keeps its pipeline
+// going from one to the next.
+//   warp 8     finds the items; loads Q and blocks of 128 keys of K and V through a ring, by TMA
 //   warp 9     issues S = Q K^T (both operands in shared memory, S in TMEM) and
 //              O += P V (P in TMEM, where S was)
 //   warps 0-7  one thread per query row: read S, mask, softmax, write P in 16 bits, and
@@ -19,6 +22,11 @@
 // S of the next block overwrites P of this one: the tensor pipe runs the MMAs of a thread
 // in order, and S of a block is complete only after the O += P V before it, which is what
 // allows the softmax warps to rescale O when they hold a new S.
+//
+// The special function units take 8 cycles for a warp's 32 exponentials, as long as the
+// tensor cores for the products they belong to. So a quarter of them is computed on the
+// FMA units: 2^x = 2^i 2^f, f in [-1/2, 1/2], by the polynomial of degree 5 with the least
+// relative error (2.2e-7; fitted by Lawson's iteration), 2^i by adding i to the exponent.
 //
 // Keys past the sequence's end belong to another sequence and may hold anything: their
 // scores are masked, the O += P V steps of 16 keys past the last visible one are not
@@ -32,7 +40,7 @@
 namespace grinqh {
 namespace {
 
-constexpr int kRows = 128;    // queries of a tile
+constexpr int kRows = 128;    // rows of a tile: tokens x query heads
 constexpr int kKeys = 128;    // keys of a block
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.0f;
@@ -45,8 +53,9 @@ struct PromptArgs {
   void* out;
   float* lse;
   int total_q, total_k;
-  int seqs, heads, group;  // group: query heads of a kv head
-  float scale_log2;        // softmax scale * log2(e)
+  int seqs, heads, kv_heads, group;  // group: query heads of a kv head
+  int tokens;                        // of a tile: 128 / group
+  float scale_log2;                  // softmax scale * log2(e)
 };
 
 template <int D>
@@ -58,22 +67,28 @@ struct Shape {
   static constexpr uint32_t kSmem = (2 + kStages) * kTileBytes + 1024 /*align*/ + 512 /*barriers*/;
 };
 
-// What a CTA works on.
+// Two tiles of a sequence and kv head.
 struct Item {
-  int q0, n;        // first query row, queries of the sequence
-  int k0, m;        // first key row, keys of the sequence
-  int row;          // first row of the tiles in the sequence
-  int blocks;       // key blocks the tiles see
-  bool none;
+  int q0, n;      // first query row, queries of the sequence
+  int k0, m;      // first key row, keys of the sequence
+  int token;      // first token of the tiles in the sequence
+  int kv_head;    // < 0: no more items
+  __device__ __forceinline__ int first(int t, int tokens) const { return token + t * tokens; }
+  // keys that the last token of tile t sees, and blocks of them
+  __device__ __forceinline__ int keys(int t, int tokens) const {
+    return max(0, min(m, m - n + min(n, first(t, tokens) + tokens)));
+  }
+  __device__ __forceinline__ int blocks(int t, int tokens) const {
+    return first(t, tokens) < n ? (keys(t, tokens) + kKeys - 1) / kKeys : 0;
+  }
 };
 
-// Finds row block `want` (counted from the last one) over all sequences; one warp.
-__device__ __forceinline__ Item find_item(const PromptArgs& a, int rows, int64_t want) {
+// Finds token block `want` (of `tokens` each, counted from the last one) over all sequences; one warp.
+__device__ __forceinline__ Item find_item(const PromptArgs& a, int tokens, int64_t want, int kv_head) {
   const int lane = threadIdx.x & 31;
-  Item it;
-  it.none = true;
-  // sequences from the last to the first, 32 at a time: their long rows, which see the
-  // most keys, start first
+  Item it{0, 0, 0, 0, 0, -1};
+  // sequences from the last to the first, 32 at a time, and their tokens from the last,
+  // which see the most keys
   for (int top = a.seqs; top > 0; top -= 32) {
     const int b = top - 1 - lane;
     int q0 = 0, q1 = 0;
@@ -81,7 +96,7 @@ __device__ __forceinline__ Item find_item(const PromptArgs& a, int rows, int64_t
       q0 = min(max(a.cu_q[b], 0), a.total_q);
       q1 = min(max(a.cu_q[b + 1], q0), a.total_q);
     }
-    const int count = (q1 - q0 + rows - 1) / rows;
+    const int count = (q1 - q0 + tokens - 1) / tokens;
     int upto = count;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -91,23 +106,37 @@ __device__ __forceinline__ Item find_item(const PromptArgs& a, int rows, int64_t
     const unsigned hit = __ballot_sync(0xffffffffu, want < upto);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const int first = __shfl_sync(0xffffffffu, upto - count, src);
+      const int before = __shfl_sync(0xffffffffu, upto - count, src);
       const int cnt = __shfl_sync(0xffffffffu, count, src);
+      const int bb = top - 1 - src;
       it.q0 = __shfl_sync(0xffffffffu, q0, src);
       it.n = __shfl_sync(0xffffffffu, q1, src) - it.q0;
-      it.row = (cnt - 1 - (int)(want - first)) * rows;
-      const int bb = top - 1 - src;
+      it.token = (cnt - 1 - (int)(want - before)) * tokens;
       it.k0 = min(max(a.cu_k[bb], 0), a.total_k);
       it.m = min(max(a.cu_k[bb + 1], it.k0), a.total_k) - it.k0;
-      // the last row of the tiles sees the most keys
-      const int seen = min(it.m, it.m - it.n + min(it.n, it.row + rows));
-      it.blocks = seen > 0 ? (seen + kKeys - 1) / kKeys : 0;
-      it.none = false;
+      it.kv_head = kv_head;
       return it;
     }
     want -= __shfl_sync(0xffffffffu, upto, 31);
   }
   return it;
+}
+
+// 2^x of two numbers on the FMA units; x <= 2^7, and below -126 (a masked score) it is
+// 2^-126: nothing next to the row's largest weight, which is at least 2^-kSlack.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  constexpr float kRound = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
+  const float2 f = __fadd2_rn(x, __ffma2_rn(t, make_float2(-1.f, -1.f), make_float2(kRound, kRound)));
+  float2 p = __ffma2_rn(f, make_float2(1.3276472e-3f, 1.3276472e-3f), make_float2(9.6755410e-3f, 9.6755410e-3f));
+  p = __ffma2_rn(p, f, make_float2(5.5507131e-2f, 5.5507131e-2f));
+  p = __ffma2_rn(p, f, make_float2(2.4022120e-1f, 2.4022120e-1f));
+  p = __ffma2_rn(p, f, make_float2(6.9314694e-1f, 6.9314694e-1f));
+  p = __ffma2_rn(p, f, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 template <typename T>
@@ -133,24 +162,23 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   unsigned char* s_q = smem;
   unsigned char* s_kv = smem + 2 * S::kTileBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_kv + S::kStages * S::kTileBytes);
-  uint64_t* full = bars;                      // ring stage holds its block
-  uint64_t* empty = full + S::kStages;        // ring stage may be filled
-  uint64_t* q_full = empty + S::kStages;
-  uint64_t* s_full = q_full + 1;              // [2] S of a tile is in TMEM
-  uint64_t* p_full = s_full + 2;              // [2] P of a tile is in TMEM
-  uint64_t* o_full = p_full + 2;              // [2] O of a tile is final
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
-  Item* s_item = reinterpret_cast<Item*>(tmem_slot + 2);
+  uint64_t* full = bars;                  // ring stage holds its block
+  uint64_t* empty = full + S::kStages;    // ring stage may be filled
+  uint64_t* q_full = empty + S::kStages;  // the item's queries are there
+  uint64_t* q_empty = q_full + 1;         // ... are not needed any more
+  uint64_t* s_full = q_empty + 1;         // [2] S of a tile is in TMEM
+  uint64_t* p_full = s_full + 2;          // [2][2] half of a tile's P is in TMEM
+  uint64_t* o_full = p_full + 4;          // [2] O of a tile is final
+  uint64_t* o_empty = o_full + 2;         // [2] ... is read
+  uint64_t* i_full = o_empty + 2;         // [2] an item is known
+  uint64_t* i_empty = i_full + 2;         // [2] ... is not needed any more
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
+  uint64_t* c_full = reinterpret_cast<uint64_t*>(tmem_slot + 2);  // the answer about a next CTA is there
+  Item* s_item = reinterpret_cast<Item*>(c_full + 1);             // [2]
+  __shared__ __align__(16) uint32_t s_next[4];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool paired = (a.group & 1) == 0;  // the tiles are two heads (else two row tiles)
-  const int columns = paired ? a.heads / 2 : a.heads;  // CTAs of a row block
-  const int head = (int)(blockIdx.x % columns) * (paired ? 2 : 1);
-
-  if (warp == 8) {
-    const Item it = find_item(a, paired ? kRows : 2 * kRows, blockIdx.x / columns);
-    if (lane == 0) *s_item = it;
-  } else if (warp == 9) {
+  if (warp == 9) {
     tmem_alloc(tmem_slot, kTmemCols);
   } else if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
@@ -158,47 +186,86 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       mbar_init(&empty[s], 1);
     }
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 128);
+      mbar_init(&p_full[2 * t], 128);
+      mbar_init(&p_full[2 * t + 1], 128);
       mbar_init(&o_full[t], 1);
+      mbar_init(&o_empty[t], 128);
+      mbar_init(&i_full[t], 1);
+      mbar_init(&i_empty[t], 9);
     }
+    mbar_init(c_full, 1);
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const Item it = *s_item;
-  const int kv_head = head / a.group;
-  const int nb = it.none ? 0 : it.blocks;
-  // keys that the last row of a tile sees (tile 1 of an unpaired item is 128 rows on)
-  auto tile_row = [&](int t) { return it.row + (paired ? 0 : t * kRows); };
-  auto tile_keys = [&](int t) { return min(it.m, it.m - it.n + min(it.n, tile_row(t) + kRows)); };
+  const int tokens = a.tokens;
+  // the k-th item of this CTA, for every warp but the one that finds it
+  auto item = [&](int k) {
+    mbar_wait_nocall(&i_full[k & 1], (k >> 1) & 1);
+    const Item it = s_item[k & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[k & 1]);
+    return it;
+  };
 
   // The softmax warps take the registers that the others do not need:
-  // 256 x 232 + 128 x 40 = 384 x 168, what the launch holds.
+  // 256 x 208 + 128 x 88 = 384 x 168, what the launch holds.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 8 && nb > 0) {
-      // ------------------------------------------------------------ TMA producer
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, 2 * S::kTileBytes);
-        for (int t = 0; t < 2; ++t)
-          for (int c = 0; c < S::kAtoms; ++c)
-            tma_load_3d(s_q + t * S::kTileBytes + c * S::kAtom, &tmap_q, 64 * c, paired ? head + t : head,
-                        it.q0 + tile_row(t), q_full);
-        for (int i = 0; i < 2 * nb; ++i) {  // K of block 0, V of block 0, K of block 1, ...
-          const int s = i % S::kStages;
-          if (i >= S::kStages) mbar_wait_nocall(&empty[s], ((i / S::kStages) - 1) & 1);
-          mbar_arrive_expect_tx(&full[s], S::kTileBytes);
-          for (int c = 0; c < S::kAtoms; ++c)
-            tma_load_3d(s_kv + s * S::kTileBytes + c * S::kAtom, i & 1 ? &tmap_v : &tmap_k, 64 * c, kv_head,
-                        it.k0 + (i >> 1) * kKeys, &full[s]);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
+      // ---------------------------------------------------------- items, TMA producer
+      int i = 0, used = 0;  // blocks and items loaded so far
+      int64_t at = blockIdx.x;
+      for (int k = 0;; ++k) {
+        Item it{0, 0, 0, 0, 0, -1};
+        if (at >= 0) it = find_item(a, 2 * tokens, at / a.kv_heads, (int)(at % a.kv_heads));
+        if (k >= 2) mbar_wait_nocall(&i_empty[k & 1], ((k >> 1) - 1) & 1);
+        if (lane == 0) {
+          s_item[k & 1] = it;
+          mbar_arrive(&i_full[k & 1]);
         }
+        __syncwarp();
+        if (it.kv_head < 0) break;
+        const int nb = max(it.blocks(0, tokens), it.blocks(1, tokens));
+        if (nb > 0) {
+          if (lane == 0) {
+            if (used > 0) mbar_wait_nocall(q_empty, (used - 1) & 1);
+            const uint32_t bytes = a.group * tokens * 128;  // of 64 channels of a tile
+            mbar_arrive_expect_tx(q_full, 2 * S::kAtoms * bytes);
+            for (int t = 0; t < 2; ++t)
+              for (int c = 0; c < S::kAtoms; ++c)
+                tma_load_3d(s_q + t * S::kTileBytes + c * S::kAtom, &tmap_q, 64 * c, it.kv_head * a.group,
+                            it.q0 + it.first(t, tokens), q_full);
+            for (int e = i + 2 * nb, n = i; n < e; ++n) {  // K of block 0, V of block 0, K of block 1, ...
+              const int s = n % S::kStages;
+              if (n >= S::kStages) mbar_wait_nocall(&empty[s], ((n / S::kStages) - 1) & 1);
+              mbar_arrive_expect_tx(&full[s], S::kTileBytes);
+              for (int c = 0; c < S::kAtoms; ++c)
+                tma_load_3d(s_kv + s * S::kTileBytes + c * S::kAtom, (n - i) & 1 ? &tmap_v : &tmap_k, 64 * c,
+                            it.kv_head, it.k0 + ((n - i) >> 1) * kKeys, &full[s]);
+            }
+          }
+          i += 2 * nb;
+          ++used;
+          __syncwarp();
+        }
+        // the next item is asked for only now: an SM that is behind takes fewer
+        if (lane == 0) {
+          fence_proxy_async_smem();  // the last answer has been read
+          mbar_arrive_expect_tx(c_full, 16);
+          next_cta_ask(s_next, c_full);
+        }
+        const bool answered = mbar_wait_nocall(c_full, k & 1);
+        at = answered ? next_cta_answer(s_next) : -1;
+        __syncwarp();
       }
-    } else if (warp == 9 && nb > 0) {
-      // ------------------------------------------------------------ MMA issuer
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- MMA issuer
       constexpr uint32_t fmt = Act<T>::kBf16 ? 1 : 0;
       constexpr uint32_t id_s = instr_desc(1, fmt, fmt, 0, 0, kKeys, kRows);
       constexpr uint32_t id_o = instr_desc(1, fmt, fmt, 0, 1, D, kRows);
@@ -211,76 +278,103 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         }
         mma_commit(&s_full[t]);
       };
-      auto outputs = [&](int t, int j, int stage) {  // O_t += P_t V
-        const uint32_t vb = smem_u32(s_kv + stage * S::kTileBytes);
-        const int steps = min(kKeys / 16, (tile_keys(t) - j * kKeys + 15) / 16);
-        for (int kk = 0; kk < steps; ++kk)
+      auto outputs = [&](int t, uint32_t vb, int from, int to, bool more) {  // O_t += P_t V, steps of 16 keys
+        for (int kk = from; kk < to; ++kk)
           mma_f16_ts(tmem + kTmemO + t * 128, tmem + t * kKeys + kk * 8, smem_desc(vb + kk * 2048, S::kAtom, 1024, 2),
-                     id_o, (j > 0 || kk > 0) ? 1u : 0u);
+                     id_o, (more || kk > 0) ? 1u : 0u);
       };
-      mbar_wait_nocall(q_full, 0);
-      mbar_wait_nocall(&full[0], 0);
-      if (lane == 0) {
-        scores(0, 0);
-        scores(1, 0);
-        mma_commit(&empty[0]);
-      }
-      __syncwarp();
-      for (int j = 0; j < nb; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 2;
-        const int vs = vi % S::kStages, ks = ki % S::kStages;
-        mbar_wait_nocall(&full[vs], (vi / S::kStages) & 1);
-        const int left = it.m - j * kKeys;  // keys of the sequence from this block on
-        if (left < kKeys && (left & 15)) {
-          // rows of V behind the sequence's end in its last step of 16 keys
-          for (int r = left + (lane >> 3); r < ((left + 15) & ~15); r += 4)
-            for (int c = 0; c < S::kAtoms; ++c)
-              *reinterpret_cast<uint4*>(s_kv + vs * S::kTileBytes + c * S::kAtom + r * 128 + (lane & 7) * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_smem();
-          __syncwarp();
+      int i = 0, used = 0;    // blocks and items so far
+      int np[2] = {0, 0}, no[2] = {0, 0};  // halves of P and outputs of each tile so far
+      for (int k = 0;; ++k) {
+        const Item it = item(k);
+        if (it.kv_head < 0) break;
+        const int nbt[2] = {it.blocks(0, tokens), it.blocks(1, tokens)};
+        const int nb = max(nbt[0], nbt[1]);
+        if (nb == 0) continue;
+        mbar_wait_nocall(q_full, used & 1);
+        mbar_wait_nocall(&full[i % S::kStages], (i / S::kStages) & 1);
+        if (lane == 0) {
+          for (int t = 0; t < 2; ++t)
+            if (nbt[t] > 0) scores(t, i % S::kStages);
+          mma_commit(&empty[i % S::kStages]);
+          if (nb == 1) mma_commit(q_empty);
         }
-        for (int t = 0; t < 2; ++t) {
-          mbar_wait_nocall(&p_full[t], j & 1);
-          tc_fence_after();
-          if (t == 0 && j + 1 < nb) mbar_wait_nocall(&full[ks], (ki / S::kStages) & 1);
-          if (lane == 0) {
-            outputs(t, j, vs);
-            if (j + 1 < nb) {
-              scores(t, ks);
-            } else {
-              mma_commit(&o_full[t]);
+        __syncwarp();
+        for (int j = 0; j < nb; ++j) {
+          const int vi = i + 2 * j + 1, ki = vi + 1;
+          const int vs = vi % S::kStages, ks = ki % S::kStages;
+          const uint32_t vb = smem_u32(s_kv + vs * S::kTileBytes);
+          mbar_wait_nocall(&full[vs], (vi / S::kStages) & 1);
+          const int left = it.m - j * kKeys;  // keys of the sequence from this block on
+          if (left < kKeys && (left & 15)) {
+            // rows of V behind the sequence's end in its last step of 16 keys
+            for (int r = left + (lane >> 3); r < ((left + 15) & ~15); r += 4)
+              for (int c = 0; c < S::kAtoms; ++c)
+                *reinterpret_cast<uint4*>(s_kv + vs * S::kTileBytes + c * S::kAtom + r * 128 + (lane & 7) * 16) =
+                    make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (j + 1 < nb) mbar_wait_nocall(&full[ks], (ki / S::kStages) & 1);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= nbt[t]) continue;
+            const int steps = min(kKeys / 16, (it.keys(t, tokens) - j * kKeys + 15) / 16);
+            if (j == 0 && no[t] > 0) mbar_wait_nocall(&o_empty[t], (no[t] - 1) & 1);
+            mbar_wait_nocall(&p_full[2 * t], np[t] & 1);
+            tc_fence_after();
+            if (lane == 0) outputs(t, vb, 0, min(steps, 4), j > 0);
+            __syncwarp();
+            mbar_wait_nocall(&p_full[2 * t + 1], np[t] & 1);
+            tc_fence_after();
+            ++np[t];
+            if (lane == 0) {
+              outputs(t, vb, 4, steps, true);
+              if (j + 1 < nbt[t])
+                scores(t, ks);
+              else
+                mma_commit(&o_full[t]);
             }
+            if (j + 1 == nbt[t]) ++no[t];
+            __syncwarp();
+          }
+          if (lane == 0) {
+            mma_commit(&empty[vs]);
+            if (j + 1 < nb) mma_commit(&empty[ks]);
+            if (j + 2 == nb) mma_commit(q_empty);  // the last scores are under way
           }
           __syncwarp();
         }
-        if (lane == 0) {
-          mma_commit(&empty[vs]);
-          if (j + 1 < nb) mma_commit(&empty[ks]);
-        }
-        __syncwarp();
+        i += 2 * nb;
+        ++used;
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-    if (!it.none) {
-      // ------------------------------------------------------------ softmax, epilogue
-      const int t = warp >> 2;
-      const int r = (warp & 3) * 32 + lane;           // row of the tile
-      const int row = tile_row(t) + r;                // of the sequence
-      const int seen = min(it.m, it.m - it.n + row + 1);  // keys this row sees (<= 0: none)
-      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t ts = tmem + lanes + t * kKeys, to = tmem + lanes + kTmemO + t * 128;
-      const int first_seen = it.m - it.n + tile_row(t) + 1;  // keys the tile's first row sees
-      float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < nb; ++j) {
-        mbar_wait_nocall(&s_full[t], j & 1);
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ------------------------------------------------------------ softmax, epilogue
+    const int t = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;  // row of the tile
+    const int r_token = r / a.group, r_head = r - r_token * a.group;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + t * kKeys, to = tmem + lanes + kTmemO + t * 128;
+    int ns = 0, no = 0;  // blocks and outputs so far
+    for (int k = 0;; ++k) {
+      const Item it = item(k);
+      if (it.kv_head < 0) break;
+      const int nb = it.blocks(t, tokens);
+      const int token = it.first(t, tokens) + r_token;         // of the sequence
+      const int seen = min(it.m, it.m - it.n + token + 1);      // keys this row sees (<= 0: none)
+      const int all_see = min(it.m, it.m - it.n + it.first(t, tokens) + 1);  // keys that every row sees
+      float m = -INFINITY, ref = 0.f;
+      float2 l0 = make_float2(0.f, 0.f), l1 = l0;
+      for (int j = 0; j < nb; ++j, ++ns) {
+        mbar_wait_nocall(&s_full[t], ns & 1);
         tc_fence_after();
         uint32_t sr[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, sr[c]);
         tmem_ld_wait();
-        if ((j + 1) * kKeys > min(it.m, first_seen)) {
+        if ((j + 1) * kKeys > all_see) {
           const int lim = seen - j * kKeys;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -288,17 +382,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             for (int i = 0; i < 32; ++i)
               if (32 * c + i >= lim) sr[c][i] = 0xff800000u;  // -inf
         }
-        float top = -INFINITY;
+        float mx[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = __uint_as_float(sr[c][0]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(sr[c][i]));
-        top *= a.scale_log2;
+          for (int i = 1; i < 31; i += 2)
+            mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(sr[c][i])), __uint_as_float(sr[c][i + 1]));
+          mx[c] = fmaxf(mx[c], __uint_as_float(sr[c][31]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
         const bool up = top > m + kSlack || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, up)) {
           const float f = up ? exp2_fast(m - top) : 1.0f;
-          if (up) m = top;
-          l *= f;
+          if (up) m = ref = top;
+          l0.x *= f, l0.y *= f, l1.x *= f, l1.y *= f;
           if (j > 0) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -311,37 +409,54 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             }
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float p0 = exp2_fast(fmaf(__uint_as_float(sr[c][2 * i]), a.scale_log2, -ref));
-            const float p1 = exp2_fast(fmaf(__uint_as_float(sr[c][2 * i + 1]), a.scale_log2, -ref));
-            l += p0 + p1;
-            pk[i] = pack2<T>(p0, p1);
+            const float2 x = __ffma2_rn(
+                make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), scale2, ref2);
+            float2 p;
+            if (i % 4 == 3) {
+              p = exp2_poly(x);
+            } else {
+              p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+            }
+            if (i & 1)
+              l1 = __fadd2_rn(l1, p);
+            else
+              l0 = __fadd2_rn(l0, p);
+            pk[i] = pack2<T>(p.x, p.y);
           }
           tmem_st16(ts + 16 * c, pk);
+          if (c & 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&p_full[2 * t + (c >> 1)]);
+          }
         }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_full[t]);
       }
-      if (nb > 0) {
-        mbar_wait_nocall(&o_full[t], 0);
-        tc_fence_after();
-      }
-      const bool in = row < it.n, none = l == 0.f;
-      const int64_t at = (int64_t)(it.q0 + row) * a.heads + (paired ? head + t : head);
+      const float l = (l0.x + l0.y) + (l1.x + l1.y);
+      const bool in = token < it.n && r_token < tokens, none = m == -INFINITY && l == l;  // no score but -inf
+      const int64_t at = (int64_t)(it.q0 + token) * a.heads + it.kv_head * a.group + r_head;
       T* out = static_cast<T*>(a.out) + at * D;
       const float inv = 1.0f / l;
+      if (nb > 0) {
+        mbar_wait_nocall(&o_full[t], no & 1);
+        tc_fence_after();
+        ++no;
+      }
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         if (nb > 0) {
           tmem_ld32(to + 32 * c, o);
           tmem_ld_wait();
+          if (c == D / 32 - 1) {
+            tc_fence_before();
+            mbar_arrive(&o_empty[t]);
+          }
         }
         if (in) {
 #pragma unroll
@@ -357,26 +472,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         __syncwarp();
       }
       if (in) a.lse[at] = none ? -INFINITY : m * kLn2 + logf(l);
-      tc_fence_before();
     }
   }
+  tc_fence_before();
   __syncthreads();
   if (warp == 9) tmem_dealloc(tmem, kTmemCols);
 }
 
 template <typename T, int D>
-int launch(const PromptArgs& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t st) {
+int launch(const PromptArgs& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
+           cudaStream_t st) {
   auto kern = prompt_attention_kernel<T, D>;
   const cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<D>::kSmem);
   if (e != cudaSuccess) return set_error(GRINQH_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  const bool paired = (a.group & 1) == 0;
-  const int rows = paired ? kRows : 2 * kRows;
-  // every sequence's rows fill whole tiles but its last: at most this many row blocks
-  const int64_t blocks = std::min<int64_t>(a.total_q / rows + a.seqs, a.total_q);
-  const int64_t grid = blocks * (paired ? a.heads / 2 : a.heads);
-  GRINQH_REQUIRE(grid < (1LL << 31), "too many row blocks (%lld)", (long long)blocks);
-  kern<<<(unsigned)grid, kThreads, Shape<D>::kSmem, st>>>(q, k, v, a);
+  // every sequence's tokens fill whole items but its last: at most this many
+  const int64_t items = std::min<int64_t>(a.total_q / (2 * a.tokens) + a.seqs, a.total_q) * a.kv_heads;
+  GRINQH_REQUIRE(items < (1LL << 31), "too many row blocks (%lld)", (long long)items);
+  kern<<<(unsigned)items, kThreads, Shape<D>::kSmem, st>>>(q, k, v, a);
   return check_launch("prompt_attention");
 }
 
@@ -414,18 +527,25 @@ extern "C" int grinqh_prompt_attention(const void* q, const void* k, const void*
                      q_head_stride % 8 == 0 && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
                      v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
                  "q, k, v, their strides and out must be 16-byte aligned");
-  const PromptArgs a{cu_seqlens_q,   cu_seqlens_k, out, lse, (int)total_q, (int)total_k, num_seqs, num_heads,
-                     num_heads / num_kv_heads, softmax_scale * 1.4426950408889634f};
+  const int group = num_heads / num_kv_heads;
+  if (group > kRows)
+    return set_error(GRINQH_ERR_UNSUPPORTED, "at most %d query heads per kv head (got %d)", kRows, group);
+  const PromptArgs a{cu_seqlens_q, cu_seqlens_k, out,          lse,   (int)total_q,  (int)total_k,
+                     num_seqs,     num_heads,    num_kv_heads, group, kRows / group, softmax_scale * 1.4426950408889634f};
   const bool bf16 = dtype == GRINQH_BF16;
   CUtensorMap tq, tk, tv;
-  GRINQH_RETURN_IF(tmap_heads(&tq, bf16, q, total_q, num_heads, head_dim, q_token_stride, q_head_stride, 128, "q"));
+  GRINQH_RETURN_IF(tmap_heads(&tq, bf16, q, total_q, num_heads, head_dim, q_token_stride, q_head_stride, group,
+                              a.tokens, "q"));
   if (total_k > 0) {
-    GRINQH_RETURN_IF(tmap_heads(&tk, bf16, k, total_k, num_kv_heads, head_dim, k_token_stride, k_head_stride, 128, "k"));
-    GRINQH_RETURN_IF(tmap_heads(&tv, bf16, v, total_k, num_kv_heads, head_dim, v_token_stride, v_head_stride, 128, "v"));
+    GRINQH_RETURN_IF(tmap_heads(&tk, bf16, k, total_k, num_kv_heads, head_dim, k_token_stride, k_head_stride, 1, kKeys,
+                                "k"));
+    GRINQH_RETURN_IF(tmap_heads(&tv, bf16, v, total_k, num_kv_heads, head_dim, v_token_stride, v_head_stride, 1, kKeys,
+                                "v"));
   } else {
     tk = tv = tq;  // never read: no row sees a key
   }
   if (head_dim == 128)
-    return bf16 ? launch<__nv_bfloat16, 128>(a, tq, tk, tv, stream) : launch<__half, 128>(a, tq, tk, tv, stream);
+    return bf16 ? launch<__nv_bfloat16, 128>(a, tq, tk, tv, stream)
+                : launch<__half, 128>(a, tq, tk, tv, stream);
   return bf16 ? launch<__nv_bfloat16, 64>(a, tq, tk, tv, stream) : launch<__half, 64>(a, tq, tk, tv, stream);
 }

@@ -376,6 +376,29 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
+// ---------------------------------------------------------------- launch control
+// Asks for a CTA of this grid that has not started: 16 bytes of answer to `dst` (16-byte
+// aligned shared memory), completion counted on `bar`. After a refusal no more is asked.
+__device__ __forceinline__ void next_cta_ask(void* dst, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(dst)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+
+// The answer: that CTA's blockIdx.x, which this CTA now does the work of, or -1.
+__device__ __forceinline__ int64_t next_cta_answer(const void* src) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(src))
+      : "memory");
+  return ok ? (int64_t)x : -1;
+}
+
 __device__ __forceinline__ void named_barrier(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }

@@ -23,10 +23,11 @@ inline EncodeTiledFn tmap_encoder() {
   return fn;
 }
 
-// Rows of 16-bit heads [tokens, heads, dim] (strides in elements) as boxes of 64 channels
-// of one head x `rows` tokens, 128-byte swizzle; tokens past the end read as zero.
+// 16-bit heads [tokens, heads, dim] (strides in elements) as boxes of 64 channels x
+// `box_heads` x `box_tokens`, 128-byte swizzle; tokens past the end read as zero.
 inline int tmap_heads(CUtensorMap* map, bool bf16, const void* base, int64_t tokens, int64_t heads, int64_t dim,
-                      int64_t token_stride, int64_t head_stride, uint32_t rows, const char* what) {
+                      int64_t token_stride, int64_t head_stride, uint32_t box_heads, uint32_t box_tokens,
+                      const char* what) {
   const EncodeTiledFn enc = tmap_encoder();
   if (!enc) return set_error(GRINQH_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   // a stride that no index is multiplied with may hold anything
@@ -34,7 +35,7 @@ inline int tmap_heads(CUtensorMap* map, bool bf16, const void* base, int64_t tok
   if (tokens == 1) token_stride = heads * dim;
   const cuuint64_t gdim[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
   const cuuint64_t gstride[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
-  const cuuint32_t box[3] = {64, 1, rows}, step[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, box_heads, box_tokens}, step[3] = {1, 1, 1};
   const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                          const_cast<void*>(base), gdim, gstride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
