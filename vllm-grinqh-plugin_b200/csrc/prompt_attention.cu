@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   Item* s_item = reinterpret_cast<Item*>(c_full + 1);             // [2]
   __shared__ __align__(16) uint32_t s_next[4];
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == 9) {
     tmem_alloc(tmem_slot, kTmemCols);
   } else if (threadIdx.x == 0) {
@@ -269,43 +269,61 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       constexpr uint32_t fmt = Act<T>::kBf16 ? 1 : 0;
       constexpr uint32_t id_s = instr_desc(1, fmt, fmt, 0, 0, kKeys, kRows);
       constexpr uint32_t id_o = instr_desc(1, fmt, fmt, 0, 1, D, kRows);
+      constexpr uint32_t kTile16 = S::kTileBytes >> 4, kAtom16 = S::kAtom >> 4;
+      const uint32_t go = lane == 0;
+      const uint32_t tm = uniform(tmem);
+      // descriptors by their first one: an address is 16 bytes a unit, in the low bits
+      const uint64_t q_desc = smem_desc(smem_u32(s_q), 16, 1024, 2);
+      const uint64_t k_desc = smem_desc(smem_u32(s_kv), 16, 1024, 2);
+      const uint64_t v_desc = smem_desc(smem_u32(s_kv), S::kAtom, 1024, 2);
       auto scores = [&](int t, int stage) {  // S_t = Q_t K^T
-        const uint32_t qb = smem_u32(s_q + t * S::kTileBytes), kb = smem_u32(s_kv + stage * S::kTileBytes);
+        const uint64_t qd = q_desc + t * kTile16, kd = k_desc + stage * kTile16;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4) * S::kAtom + (kk % 4) * 32;
-          mma_f16_ss(tmem + t * kKeys, smem_desc(qb + off, 16, 1024, 2), smem_desc(kb + off, 16, 1024, 2), id_s, kk > 0);
+          const uint32_t off = (kk / 4) * kAtom16 + (kk % 4) * 2;
+          mma_f16_ss_if(go, tm + t * kKeys, qd + off, kd + off, id_s, kk > 0);
         }
-        mma_commit(&s_full[t]);
+        mma_commit_if(go, &s_full[t]);
       };
-      auto outputs = [&](int t, uint32_t vb, int from, int to, bool more) {  // O_t += P_t V, steps of 16 keys
-        for (int kk = from; kk < to; ++kk)
-          mma_f16_ts(tmem + kTmemO + t * 128, tmem + t * kKeys + kk * 8, smem_desc(vb + kk * 2048, S::kAtom, 1024, 2),
-                     id_o, (more || kk > 0) ? 1u : 0u);
+      auto outputs = [&](int t, int stage, int from, int steps, bool more) {  // O_t += P_t V, steps of 16 keys
+        const uint64_t vd = v_desc + stage * kTile16;
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const int kk = from + k4;
+          if (kk < steps)
+            mma_f16_ts_if(go, tm + kTmemO + t * 128, tm + t * kKeys + kk * 8, vd + kk * 128, id_o,
+                          more || kk > 0 ? 1u : 0u);
+        }
       };
-      int i = 0, used = 0;    // blocks and items so far
-      int np[2] = {0, 0}, no[2] = {0, 0};  // halves of P and outputs of each tile so far
+      int stage = 0, round = 0, used = 0;  // ring stage of the next block and its parity; items so far
+      auto next = [&] {
+        if (++stage == S::kStages) {
+          stage = 0;
+          round ^= 1;
+        }
+      };
+      int np[2] = {0, 0}, no[2] = {0, 0};  // blocks and outputs of each tile so far
       for (int k = 0;; ++k) {
         const Item it = item(k);
-        if (it.kv_head < 0) break;
-        const int nbt[2] = {it.blocks(0, tokens), it.blocks(1, tokens)};
-        const int nb = max(nbt[0], nbt[1]);
+        if (uniform(it.kv_head) < 0) break;
+        const int nbt[2] = {uniform(it.blocks(0, tokens)), uniform(it.blocks(1, tokens))};
+        const int keys[2] = {uniform(it.keys(0, tokens)), uniform(it.keys(1, tokens))};
+        const int nb = max(nbt[0], nbt[1]), m = uniform(it.m);
         if (nb == 0) continue;
         mbar_wait_nocall(q_full, used & 1);
-        mbar_wait_nocall(&full[i % S::kStages], (i / S::kStages) & 1);
-        if (lane == 0) {
-          for (int t = 0; t < 2; ++t)
-            if (nbt[t] > 0) scores(t, i % S::kStages);
-          mma_commit(&empty[i % S::kStages]);
-          if (nb == 1) mma_commit(q_empty);
-        }
-        __syncwarp();
+        mbar_wait_nocall(&full[stage], round);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (nbt[t] > 0) scores(t, stage);
+        mma_commit_if(go, &empty[stage]);
+        if (nb == 1) mma_commit_if(go, q_empty);
+        next();
         for (int j = 0; j < nb; ++j) {
-          const int vi = i + 2 * j + 1, ki = vi + 1;
-          const int vs = vi % S::kStages, ks = ki % S::kStages;
-          const uint32_t vb = smem_u32(s_kv + vs * S::kTileBytes);
-          mbar_wait_nocall(&full[vs], (vi / S::kStages) & 1);
-          const int left = it.m - j * kKeys;  // keys of the sequence from this block on
+          const int vs = stage;
+          mbar_wait_nocall(&full[vs], round);
+          next();
+          const int ks = stage;
+          const int left = m - j * kKeys;  // keys of the sequence from this block on
           if (left < kKeys && (left & 15)) {
             // rows of V behind the sequence's end in its last step of 16 keys
             for (int r = left + (lane >> 3); r < ((left + 15) & ~15); r += 4)
@@ -315,37 +333,33 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             fence_proxy_async_smem();
             __syncwarp();
           }
-          if (j + 1 < nb) mbar_wait_nocall(&full[ks], (ki / S::kStages) & 1);
+          if (j + 1 < nb) {
+            mbar_wait_nocall(&full[ks], round);
+            next();
+          }
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (j >= nbt[t]) continue;
-            const int steps = min(kKeys / 16, (it.keys(t, tokens) - j * kKeys + 15) / 16);
+            const int steps = min(kKeys / 16, (keys[t] - j * kKeys + 15) / 16);
             if (j == 0 && no[t] > 0) mbar_wait_nocall(&o_empty[t], (no[t] - 1) & 1);
             mbar_wait_nocall(&p_full[2 * t], np[t] & 1);
             tc_fence_after();
-            if (lane == 0) outputs(t, vb, 0, min(steps, 4), j > 0);
-            __syncwarp();
+            outputs(t, vs, 0, steps, j > 0);
             mbar_wait_nocall(&p_full[2 * t + 1], np[t] & 1);
             tc_fence_after();
             ++np[t];
-            if (lane == 0) {
-              outputs(t, vb, 4, steps, true);
-              if (j + 1 < nbt[t])
-                scores(t, ks);
-              else
-                mma_commit(&o_full[t]);
+            outputs(t, vs, 4, steps, true);
+            if (j + 1 < nbt[t]) {
+              scores(t, ks);
+            } else {
+              mma_commit_if(go, &o_full[t]);
+              ++no[t];
             }
-            if (j + 1 == nbt[t]) ++no[t];
-            __syncwarp();
           }
-          if (lane == 0) {
-            mma_commit(&empty[vs]);
-            if (j + 1 < nb) mma_commit(&empty[ks]);
-            if (j + 2 == nb) mma_commit(q_empty);  // the last scores are under way
-          }
-          __syncwarp();
+          mma_commit_if(go, &empty[vs]);
+          if (j + 1 < nb) mma_commit_if(go, &empty[ks]);
+          if (j + 2 == nb) mma_commit_if(go, q_empty);  // the last scores are under way
         }
-        i += 2 * nb;
         ++used;
       }
     }
