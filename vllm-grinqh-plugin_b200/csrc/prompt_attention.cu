@@ -3,9 +3,9 @@
 //   s = scale * q k^T over the keys a query sees, p = softmax(s), out = p v
 //
 // One pass over the keys with the running maximum m and sum l of the softmax: a block of
-// 128 keys adds exp2(s' - m) v to an accumulator, s' = s log2(e). m is kept where a new
-// maximum exceeds it by less than kSlack: the weights then reach at most 2^kSlack, no
-// accumulator is rescaled, and the division by l in the end makes up for it.
+// keys adds exp2(s' - m) v to an accumulator, s' = s log2(e). m is kept where a new maximum
+// exceeds it by less than kSlack: the weights then reach at most 2^kSlack, no accumulator
+// is rescaled, and the division by l in the end makes up for it.
 //
 // A tile is 128 rows: as many tokens as its query heads of one kv head allow, token by
 // token (which a TMA box of {64 channels, heads, tokens} lays out by itself), so a short
@@ -14,19 +14,19 @@
 // per item, those that see the most keys first; the CTA that an SM runs takes over the
 // items of CTAs that have not started (cluster launch control) and keeps its pipeline
 // going from one to the next.
-//   warp 8     finds the items; loads Q and blocks of 128 keys of K and V through a ring, by TMA
+//   warp 8     finds the items; loads Q and blocks of K and V through a ring, by TMA
 //   warp 9     issues S = Q K^T (both operands in shared memory, S in TMEM) and
-//              O += P V (P in TMEM, where S was)
+//              O += P V (P in TMEM)
 //   warps 0-7  one thread per query row: read S, mask, softmax, write P in 16 bits, and
 //              at the end read O, divide and store
-// S of the next block overwrites P of this one: the tensor pipe runs the MMAs of a thread
-// in order, and S of a block is complete only after the O += P V before it, which is what
-// allows the softmax warps to rescale O when they hold a new S.
-//
-// The special function units take 8 cycles for a warp's 32 exponentials, as long as the
-// tensor cores for the products they belong to. So a quarter of them is computed on the
-// FMA units: 2^x = 2^i 2^f, f in [-1/2, 1/2], by the polynomial of degree 5 with the least
-// relative error (2.2e-7; fitted by Lawson's iteration), 2^i by adding i to the exponent.
+// The softmax warps hold a block's scores, then its weights, in registers: S is free for
+// the other tile as soon as it is read, and P (and O) may be in use until the next weights
+// are made. So one S serves both tiles, S, P and O fit the 512 columns of TMEM, and the
+// products follow one another as S0 O0 S1 O1, each with a whole round of the others to
+// wait in. A 128 x 128 x 16 product takes 102 cycles with both operands in shared memory
+// and 78 with A in TMEM (measured alone; 64 would be full rate), 2880 a round at head_dim
+// 128: that is what bounds the kernel there, and the exponentials, 8 cycles for a warp's
+// 32 of them or 2048 a round, at head_dim 64.
 //
 // Keys past the sequence's end belong to another sequence and may hold anything: their
 // scores are masked, the O += P V steps of 16 keys past the last visible one are not
@@ -41,12 +41,10 @@ namespace grinqh {
 namespace {
 
 constexpr int kRows = 128;    // rows of a tile: tokens x query heads
-constexpr int kKeys = 128;    // keys of a block
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.0f;
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kTmemO = 256;  // columns: S0 / P0 at 0, S1 / P1 at 128, O0, O1 from here
 
 struct PromptArgs {
   const int32_t *cu_q, *cu_k;
@@ -60,11 +58,17 @@ struct PromptArgs {
 
 template <int D>
 struct Shape {
-  static constexpr int kAtoms = D / 64;                  // 64-channel (128-byte) columns of a tile
-  static constexpr uint32_t kAtom = 128 * 128;           // bytes of one, 128 rows
-  static constexpr uint32_t kTileBytes = kAtoms * kAtom;
+  static constexpr int kKeys = 128;                      // of a block
+  static constexpr int kAtoms = D / 64;                  // 64-channel (128-byte) columns of a tile or block
+  static constexpr uint32_t kQAtom = kRows * 128;        // bytes of one
+  static constexpr uint32_t kQBytes = kAtoms * kQAtom;
+  static constexpr uint32_t kAtom = kKeys * 128;
+  static constexpr uint32_t kBytes = kAtoms * kAtom;
   static constexpr int kStages = D == 128 ? 5 : 10;      // K / V blocks in the ring
-  static constexpr uint32_t kSmem = (2 + kStages) * kTileBytes + 1024 /*align*/ + 512 /*barriers*/;
+  static constexpr uint32_t kSmem = 2 * kQBytes + kStages * kBytes + 1024 /*align*/ + 512 /*barriers*/;
+  // TMEM columns: S, then P and O of both tiles
+  static constexpr uint32_t kS = 0, kP = kKeys, kO = 2 * kKeys, kPNext = kKeys / 2, kONext = D;
+  static_assert(kO + 2 * D <= kTmemCols && kSmem <= 227 * 1024, "budgets");
 };
 
 // Two tiles of a sequence and kv head.
@@ -78,8 +82,9 @@ struct Item {
   __device__ __forceinline__ int keys(int t, int tokens) const {
     return max(0, min(m, m - n + min(n, first(t, tokens) + tokens)));
   }
+  template <int KEYS>
   __device__ __forceinline__ int blocks(int t, int tokens) const {
-    return first(t, tokens) < n ? (keys(t, tokens) + kKeys - 1) / kKeys : 0;
+    return first(t, tokens) < n ? (keys(t, tokens) + KEYS - 1) / KEYS : 0;
   }
 };
 
@@ -122,23 +127,6 @@ __device__ __forceinline__ Item find_item(const PromptArgs& a, int tokens, int64
   return it;
 }
 
-// 2^x of two numbers on the FMA units; x <= 2^7, and below -126 (a masked score) it is
-// 2^-126: nothing next to the row's largest weight, which is at least 2^-kSlack.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  constexpr float kRound = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
-  const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
-  const float2 f = __fadd2_rn(x, __ffma2_rn(t, make_float2(-1.f, -1.f), make_float2(kRound, kRound)));
-  float2 p = __ffma2_rn(f, make_float2(1.3276472e-3f, 1.3276472e-3f), make_float2(9.6755410e-3f, 9.6755410e-3f));
-  p = __ffma2_rn(p, f, make_float2(5.5507131e-2f, 5.5507131e-2f));
-  p = __ffma2_rn(p, f, make_float2(2.4022120e-1f, 2.4022120e-1f));
-  p = __ffma2_rn(p, f, make_float2(6.9314694e-1f, 6.9314694e-1f));
-  p = __ffma2_rn(p, f, make_float2(1.0f, 1.0f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (Act<T>::kBf16) {
@@ -156,41 +144,43 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                                                                        const __grid_constant__ CUtensorMap tmap_v,
                                                                        const PromptArgs a) {
   using S = Shape<D>;
+  constexpr int kKeys = S::kKeys, ST = S::kStages;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* s_q = smem;
-  unsigned char* s_kv = smem + 2 * S::kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_kv + S::kStages * S::kTileBytes);
-  uint64_t* full = bars;                  // ring stage holds its block
-  uint64_t* empty = full + S::kStages;    // ring stage may be filled
-  uint64_t* q_full = empty + S::kStages;  // the item's queries are there
-  uint64_t* q_empty = q_full + 1;         // ... are not needed any more
-  uint64_t* s_full = q_empty + 1;         // [2] S of a tile is in TMEM
-  uint64_t* p_full = s_full + 2;          // [2][2] half of a tile's P is in TMEM
-  uint64_t* o_full = p_full + 4;          // [2] O of a tile is final
-  uint64_t* o_empty = o_full + 2;         // [2] ... is read
-  uint64_t* i_full = o_empty + 2;         // [2] an item is known
-  uint64_t* i_empty = i_full + 2;         // [2] ... is not needed any more
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
-  uint64_t* c_full = reinterpret_cast<uint64_t*>(tmem_slot + 2);  // the answer about a next CTA is there
-  Item* s_item = reinterpret_cast<Item*>(c_full + 1);             // [2]
+  unsigned char* s_kv = smem + 2 * S::kQBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_kv + ST * S::kBytes);
+  uint64_t* full = bars;            // ring stage holds its block
+  uint64_t* empty = full + ST;      // ring stage may be filled
+  uint64_t* q_full = empty + ST;    // the item's queries are there
+  uint64_t* q_empty = q_full + 1;   // ... are not needed any more
+  uint64_t* s_full = q_empty + 1;   // [2] S of a tile is in TMEM
+  uint64_t* s_empty = s_full + 2;   // ... is in registers
+  uint64_t* p_full = s_empty + 1;   // [2] P of a tile is in TMEM
+  uint64_t* o_full = p_full + 2;    // [2] ... has been multiplied: O holds the block, P may be written
+  uint64_t* o_empty = o_full + 2;   // [2] O of an item is read
+  uint64_t* i_full = o_empty + 2;   // [2] an item is known
+  uint64_t* i_empty = i_full + 2;   // [2] ... is not needed any more
+  uint64_t* c_full = i_empty + 2;   // the answer about a next CTA is there
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_full + 1);
+  Item* s_item = reinterpret_cast<Item*>(tmem_slot + 2);  // [2]
   __shared__ __align__(16) uint32_t s_next[4];
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == 9) {
     tmem_alloc(tmem_slot, kTmemCols);
   } else if (threadIdx.x == 0) {
-    for (int s = 0; s < S::kStages; ++s) {
+    for (int s = 0; s < ST; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
+    mbar_init(s_empty, 128);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[2 * t], 128);
-      mbar_init(&p_full[2 * t + 1], 128);
+      mbar_init(&p_full[t], 128);
       mbar_init(&o_full[t], 1);
       mbar_init(&o_empty[t], 128);
       mbar_init(&i_full[t], 1);
@@ -214,12 +204,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   };
 
   // The softmax warps take the registers that the others do not need:
-  // 256 x 208 + 128 x 88 = 384 x 168, what the launch holds.
+  // 256 x 224 + 128 x 56 = 384 x 168, what the launch holds.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 8) {
       // ---------------------------------------------------------- items, TMA producer
-      int i = 0, used = 0;  // blocks and items loaded so far
+      int stage = 0, round = 1, used = 0;  // ring stage and parity of its release; items so far
       int64_t at = blockIdx.x;
       for (int k = 0;; ++k) {
         Item it{0, 0, 0, 0, 0, -1};
@@ -231,28 +221,32 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         }
         __syncwarp();
         if (it.kv_head < 0) break;
-        const int nb = max(it.blocks(0, tokens), it.blocks(1, tokens));
+        const int nb = max(it.blocks<kKeys>(0, tokens), it.blocks<kKeys>(1, tokens));
         if (nb > 0) {
+          if (used > 0) mbar_wait_nocall(q_empty, (used - 1) & 1);
+          ++used;
           if (lane == 0) {
-            if (used > 0) mbar_wait_nocall(q_empty, (used - 1) & 1);
             const uint32_t bytes = a.group * tokens * 128;  // of 64 channels of a tile
             mbar_arrive_expect_tx(q_full, 2 * S::kAtoms * bytes);
             for (int t = 0; t < 2; ++t)
               for (int c = 0; c < S::kAtoms; ++c)
-                tma_load_3d(s_q + t * S::kTileBytes + c * S::kAtom, &tmap_q, 64 * c, it.kv_head * a.group,
+                tma_load_3d(s_q + t * S::kQBytes + c * S::kQAtom, &tmap_q, 64 * c, it.kv_head * a.group,
                             it.q0 + it.first(t, tokens), q_full);
-            for (int e = i + 2 * nb, n = i; n < e; ++n) {  // K of block 0, V of block 0, K of block 1, ...
-              const int s = n % S::kStages;
-              if (n >= S::kStages) mbar_wait_nocall(&empty[s], ((n / S::kStages) - 1) & 1);
-              mbar_arrive_expect_tx(&full[s], S::kTileBytes);
+          }
+          for (int n = 0; n < 2 * nb; ++n) {  // K of block 0, V of block 0, K of block 1, ...
+            mbar_wait_nocall(&empty[stage], round);
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full[stage], S::kBytes);
               for (int c = 0; c < S::kAtoms; ++c)
-                tma_load_3d(s_kv + s * S::kTileBytes + c * S::kAtom, (n - i) & 1 ? &tmap_v : &tmap_k, 64 * c,
-                            it.kv_head, it.k0 + ((n - i) >> 1) * kKeys, &full[s]);
+                tma_load_3d(s_kv + stage * S::kBytes + c * S::kAtom, n & 1 ? &tmap_v : &tmap_k, 64 * c, it.kv_head,
+                            it.k0 + (n >> 1) * kKeys, &full[stage]);
+            }
+            __syncwarp();
+            if (++stage == ST) {
+              stage = 0;
+              round ^= 1;
             }
           }
-          i += 2 * nb;
-          ++used;
-          __syncwarp();
         }
         // the next item is asked for only now: an SM that is behind takes fewer
         if (lane == 0) {
@@ -269,113 +263,118 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       constexpr uint32_t fmt = Act<T>::kBf16 ? 1 : 0;
       constexpr uint32_t id_s = instr_desc(1, fmt, fmt, 0, 0, kKeys, kRows);
       constexpr uint32_t id_o = instr_desc(1, fmt, fmt, 0, 1, D, kRows);
-      constexpr uint32_t kTile16 = S::kTileBytes >> 4, kAtom16 = S::kAtom >> 4;
-      const uint32_t go = lane == 0;
       const uint32_t tm = uniform(tmem);
       // descriptors by their first one: an address is 16 bytes a unit, in the low bits
       const uint64_t q_desc = smem_desc(smem_u32(s_q), 16, 1024, 2);
       const uint64_t k_desc = smem_desc(smem_u32(s_kv), 16, 1024, 2);
       const uint64_t v_desc = smem_desc(smem_u32(s_kv), S::kAtom, 1024, 2);
-      auto scores = [&](int t, int stage) {  // S_t = Q_t K^T
-        const uint64_t qd = q_desc + t * kTile16, kd = k_desc + stage * kTile16;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4) * kAtom16 + (kk % 4) * 2;
-          mma_f16_ss_if(go, tm + t * kKeys, qd + off, kd + off, id_s, kk > 0);
-        }
-        mma_commit_if(go, &s_full[t]);
+      int ns = 0, np[2] = {0, 0}, no[2] = {0, 0};  // uses of S, weights and outputs of each tile so far
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) mma_commit(bar);
+        __syncwarp();
       };
-      auto outputs = [&](int t, int stage, int from, int steps, bool more) {  // O_t += P_t V, steps of 16 keys
-        const uint64_t vd = v_desc + stage * kTile16;
+      auto scores = [&](int t, int at) {  // S = Q_t K^T
+        if (ns > 0) mbar_wait_nocall(s_empty, (ns - 1) & 1);
+        ++ns;
+        tc_fence_after();
+        const uint64_t qd = q_desc + t * (S::kQBytes >> 4), kd = k_desc + at * (S::kBytes >> 4);
+        if (elect_one()) {
 #pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4) {
-          const int kk = from + k4;
-          if (kk < steps)
-            mma_f16_ts_if(go, tm + kTmemO + t * 128, tm + t * kKeys + kk * 8, vd + kk * 128, id_o,
-                          more || kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_f16_ss(tm + S::kS, qd + (kk / 4) * (S::kQAtom >> 4) + (kk % 4) * 2,
+                       kd + (kk / 4) * (S::kAtom >> 4) + (kk % 4) * 2, id_s, kk > 0);
+          mma_commit(&s_full[t]);
         }
+        __syncwarp();
+      };
+      auto outputs = [&](int t, int at, int steps, bool more) {  // O_t += P_t V, steps of 16 keys
+        mbar_wait_nocall(&p_full[t], np[t] & 1);
+        ++np[t];
+        tc_fence_after();
+        const uint64_t vd = v_desc + at * (S::kBytes >> 4);
+        const uint32_t o = tm + S::kO + t * S::kONext, p = tm + S::kP + t * S::kPNext;
+        if (elect_one()) {
+          if (steps == kKeys / 16) {
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              mma_f16_ts(o, p + kk * 8, vd + kk * 128, id_o, more || kk > 0 ? 1u : 0u);
+          } else {
+            for (int kk = 0; kk < steps; ++kk)
+              mma_f16_ts(o, p + kk * 8, vd + kk * 128, id_o, more || kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&o_full[t]);
+        }
+        __syncwarp();
       };
       int stage = 0, round = 0, used = 0;  // ring stage of the next block and its parity; items so far
       auto next = [&] {
-        if (++stage == S::kStages) {
+        mbar_wait_nocall(&full[stage], round);
+        const int at = stage;
+        if (++stage == ST) {
           stage = 0;
           round ^= 1;
         }
+        return at;
       };
-      int np[2] = {0, 0}, no[2] = {0, 0};  // blocks and outputs of each tile so far
       for (int k = 0;; ++k) {
         const Item it = item(k);
         if (uniform(it.kv_head) < 0) break;
-        const int nbt[2] = {uniform(it.blocks(0, tokens)), uniform(it.blocks(1, tokens))};
+        const int nbt[2] = {uniform(it.blocks<kKeys>(0, tokens)), uniform(it.blocks<kKeys>(1, tokens))};
         const int keys[2] = {uniform(it.keys(0, tokens)), uniform(it.keys(1, tokens))};
         const int nb = max(nbt[0], nbt[1]), m = uniform(it.m);
         if (nb == 0) continue;
         mbar_wait_nocall(q_full, used & 1);
-        mbar_wait_nocall(&full[stage], round);
+        ++used;
+        const int first = next();
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (nbt[t] > 0) scores(t, stage);
-        mma_commit_if(go, &empty[stage]);
-        if (nb == 1) mma_commit_if(go, q_empty);
-        next();
+          if (nbt[t] > 0) scores(t, first);
+        commit(&empty[first]);
+        if (nb == 1) commit(q_empty);
         for (int j = 0; j < nb; ++j) {
-          const int vs = stage;
-          mbar_wait_nocall(&full[vs], round);
-          next();
-          const int ks = stage;
+          const int vs = next();
           const int left = m - j * kKeys;  // keys of the sequence from this block on
           if (left < kKeys && (left & 15)) {
             // rows of V behind the sequence's end in its last step of 16 keys
             for (int r = left + (lane >> 3); r < ((left + 15) & ~15); r += 4)
               for (int c = 0; c < S::kAtoms; ++c)
-                *reinterpret_cast<uint4*>(s_kv + vs * S::kTileBytes + c * S::kAtom + r * 128 + (lane & 7) * 16) =
+                *reinterpret_cast<uint4*>(s_kv + vs * S::kBytes + c * S::kAtom + r * 128 + (lane & 7) * 16) =
                     make_uint4(0u, 0u, 0u, 0u);
             fence_proxy_async_smem();
             __syncwarp();
           }
-          if (j + 1 < nb) {
-            mbar_wait_nocall(&full[ks], round);
-            next();
-          }
+          const int ks = j + 1 < nb ? next() : 0;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
+            if (j + 1 < nbt[t]) scores(t, ks);  // of the next block, while this one's weights are made
             if (j >= nbt[t]) continue;
-            const int steps = min(kKeys / 16, (keys[t] - j * kKeys + 15) / 16);
-            if (j == 0 && no[t] > 0) mbar_wait_nocall(&o_empty[t], (no[t] - 1) & 1);
-            mbar_wait_nocall(&p_full[2 * t], np[t] & 1);
-            tc_fence_after();
-            outputs(t, vs, 0, steps, j > 0);
-            mbar_wait_nocall(&p_full[2 * t + 1], np[t] & 1);
-            tc_fence_after();
-            ++np[t];
-            outputs(t, vs, 4, steps, true);
-            if (j + 1 < nbt[t]) {
-              scores(t, ks);
-            } else {
-              mma_commit_if(go, &o_full[t]);
+            if (j == 0) {
+              if (no[t] > 0) mbar_wait_nocall(&o_empty[t], (no[t] - 1) & 1);
               ++no[t];
             }
+            outputs(t, vs, min(kKeys / 16, (keys[t] - j * kKeys + 15) / 16), j > 0);
           }
-          mma_commit_if(go, &empty[vs]);
-          if (j + 1 < nb) mma_commit_if(go, &empty[ks]);
-          if (j + 2 == nb) mma_commit_if(go, q_empty);  // the last scores are under way
+          if (j + 1 < nb) commit(&empty[ks]);
+          if (j + 2 == nb) commit(q_empty);
+          commit(&empty[vs]);
         }
-        ++used;
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ------------------------------------------------------------ softmax, epilogue
     const int t = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile
     const int r_token = r / a.group, r_head = r - r_token * a.group;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + t * kKeys, to = tmem + lanes + kTmemO + t * 128;
-    int ns = 0, no = 0;  // blocks and outputs so far
+    const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = base + S::kS, tp = base + S::kP + t * S::kPNext,
+                   to = base + S::kO + t * S::kONext;
+    constexpr int kCols = 16, kChunks = kKeys / kCols;
+    int ns = 0;  // blocks so far
     for (int k = 0;; ++k) {
       const Item it = item(k);
       if (it.kv_head < 0) break;
-      const int nb = it.blocks(t, tokens);
+      const int nb = it.blocks<kKeys>(t, tokens);
       const int token = it.first(t, tokens) + r_token;         // of the sequence
       const int seen = min(it.m, it.m - it.n + token + 1);      // keys this row sees (<= 0: none)
       const int all_see = min(it.m, it.m - it.n + it.first(t, tokens) + 1);  // keys that every row sees
@@ -384,72 +383,73 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       for (int j = 0; j < nb; ++j, ++ns) {
         mbar_wait_nocall(&s_full[t], ns & 1);
         tc_fence_after();
-        uint32_t sr[4][32];
+        uint32_t sr[kChunks][kCols];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, sr[c]);
+        for (int c = 0; c < kChunks; ++c) tmem_ld16(ts + kCols * c, sr[c]);
         tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive(s_empty);
         if ((j + 1) * kKeys > all_see) {
           const int lim = seen - j * kKeys;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (32 * c + i >= lim) sr[c][i] = 0xff800000u;  // -inf
+            for (int i = 0; i < kCols; ++i)
+              if (kCols * c + i >= lim) sr[c][i] = 0xff800000u;  // -inf
         }
-        float mx[4];
+        float mx[kChunks];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           mx[c] = __uint_as_float(sr[c][0]);
 #pragma unroll
-          for (int i = 1; i < 31; i += 2)
+          for (int i = 1; i < kCols - 1; i += 2)
             mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(sr[c][i])), __uint_as_float(sr[c][i + 1]));
-          mx[c] = fmaxf(mx[c], __uint_as_float(sr[c][31]));
+          mx[c] = fmaxf(mx[c], __uint_as_float(sr[c][kCols - 1]));
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+#pragma unroll
+        for (int c = 1; c < kChunks; ++c) mx[0] = fmaxf(mx[0], mx[c]);
+        const float top = mx[0] * a.scale_log2;
         const bool up = top > m + kSlack || (m == -INFINITY && top > m);
-        if (__any_sync(0xffffffffu, up)) {
-          const float f = up ? exp2_fast(m - top) : 1.0f;
-          if (up) m = ref = top;
-          l0.x *= f, l0.y *= f, l1.x *= f, l1.y *= f;
-          if (j > 0) {
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(to + 32 * c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st32(to + 32 * c, o);
-            }
-          }
-        }
+        const float f = up ? exp2_fast(m - top) : 1.0f;
+        if (up) m = ref = top;
+        const bool rescale = __any_sync(0xffffffffu, up);
+        if (rescale) l0.x *= f, l0.y *= f, l1.x *= f, l1.y *= f;
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
+        uint32_t pk[kChunks][kCols / 2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+        for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < kCols / 2; ++i) {
             const float2 x = __ffma2_rn(
                 make_float2(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), scale2, ref2);
-            float2 p;
-            if (i % 4 == 3) {
-              p = exp2_poly(x);
-            } else {
-              p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-            }
+            const float2 p = make_float2(exp2_fast(x.x), exp2_fast(x.y));
             if (i & 1)
               l1 = __fadd2_rn(l1, p);
             else
               l0 = __fadd2_rn(l0, p);
-            pk[i] = pack2<T>(p.x, p.y);
-          }
-          tmem_st16(ts + 16 * c, pk);
-          if (c & 1) {
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(&p_full[2 * t + (c >> 1)]);
+            pk[c][i] = pack2<T>(p.x, p.y);
           }
         }
+        // the weights stay in registers until the block before has been multiplied: P is
+        // free then, and O whole
+        if (ns > 0) mbar_wait_nocall(&o_full[t], (ns - 1) & 1);
+        tc_fence_after();
+        if (rescale && j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(to + 16 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(to + 16 * c, o);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) tmem_st8(tp + kCols / 2 * c, pk[c]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[t]);
       }
       const float l = (l0.x + l0.y) + (l1.x + l1.y);
       const bool in = token < it.n && r_token < tokens, none = m == -INFINITY && l == l;  // no score but -inf
@@ -457,9 +457,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       T* out = static_cast<T*>(a.out) + at * D;
       const float inv = 1.0f / l;
       if (nb > 0) {
-        mbar_wait_nocall(&o_full[t], no & 1);
+        mbar_wait_nocall(&o_full[t], (ns - 1) & 1);
         tc_fence_after();
-        ++no;
       }
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -547,13 +546,14 @@ extern "C" int grinqh_prompt_attention(const void* q, const void* k, const void*
   const PromptArgs a{cu_seqlens_q, cu_seqlens_k, out,          lse,   (int)total_q,  (int)total_k,
                      num_seqs,     num_heads,    num_kv_heads, group, kRows / group, softmax_scale * 1.4426950408889634f};
   const bool bf16 = dtype == GRINQH_BF16;
+  const uint32_t box = head_dim == 128 ? Shape<128>::kKeys : Shape<64>::kKeys;
   CUtensorMap tq, tk, tv;
   GRINQH_RETURN_IF(tmap_heads(&tq, bf16, q, total_q, num_heads, head_dim, q_token_stride, q_head_stride, group,
                               a.tokens, "q"));
   if (total_k > 0) {
-    GRINQH_RETURN_IF(tmap_heads(&tk, bf16, k, total_k, num_kv_heads, head_dim, k_token_stride, k_head_stride, 1, kKeys,
+    GRINQH_RETURN_IF(tmap_heads(&tk, bf16, k, total_k, num_kv_heads, head_dim, k_token_stride, k_head_stride, 1, box,
                                 "k"));
-    GRINQH_RETURN_IF(tmap_heads(&tv, bf16, v, total_k, num_kv_heads, head_dim, v_token_stride, v_head_stride, 1, kKeys,
+    GRINQH_RETURN_IF(tmap_heads(&tv, bf16, v, total_k, num_kv_heads, head_dim, v_token_stride, v_head_stride, 1, box,
                                 "v"));
   } else {
     tk = tv = tq;  // never read: no row sees a key
