@@ -328,14 +328,18 @@ int grinqh_kv4_attention(const void *q, int dtype, int64_t num_seqs, int new_tok
  * are the last of its m tokens: query j sees keys 0 .. m - n + j. Formulas, out and lse as
  * for grinqh_kv4_attention; out [total_q, num_heads, D] and lse [total_q, num_heads] are
  * contiguous, and rows that no sequence holds are not written. Strides in elements, D
- * contiguous; pointers and strides 16-byte aligned. A key or value that is not finite may
+ * contiguous; pointers and strides 16-byte aligned; at most 128 query heads per kv head.
+ * workspace: as many bytes as grinqh_prompt_attention_workspace_size says (0 where no keys
+ * are split), 256-byte aligned; its first 16 KiB are left as they are. A key or value that is not finite may
  * reach earlier queries of its own sequence (0 * inf is NaN), never another sequence. */
+size_t grinqh_prompt_attention_workspace_size(int64_t total_q, int64_t total_k, int num_seqs, int num_heads,
+                                              int num_kv_heads, int head_dim);
 int grinqh_prompt_attention(const void *q, const void *k, const void *v, int dtype, int64_t total_q, int64_t total_k,
                             int num_seqs, int num_heads, int num_kv_heads, int head_dim, int64_t q_token_stride,
                             int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
                             int64_t v_token_stride, int64_t v_head_stride, const int32_t *cu_seqlens_q,
-                            const int32_t *cu_seqlens_k, float softmax_scale, void *out, float *lse,
-                            grinqh_stream_t stream);
+                            const int32_t *cu_seqlens_k, float softmax_scale, void *out, float *lse, void *workspace,
+                            size_t workspace_bytes, grinqh_stream_t stream);
 
 #ifdef __cplusplus
 }

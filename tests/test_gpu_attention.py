@@ -308,6 +308,20 @@ def test_prompt_after_prefix_and_without_keys(dtype, dim, heads, kv):
     check_prompt(*prompt_case(nq, nk, heads, kv, dim, dtype, dim), dtype)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,heads,kv", [(128, 4, 1), (64, 3, 1), (128, 1, 1), (64, 16, 2)])
+def test_prompt_split_keys(dtype, dim, heads, kv):
+    """Few queries at the end of long keys, whose keys are worked on in parts; next to
+    sequences with hardly any keys, or none, of which some parts see nothing."""
+    nq, nk = [3, 70, 1, 130, 5], [3000, 2600, 1, 2049, 2]
+    check_prompt(*prompt_case(nq, nk, heads, kv, dim, dtype, heads), dtype)
+    q, k, v, a, b = prompt_case([40, 0], [6000, 0], heads, kv, dim, dtype, heads + 1)
+    first = check_prompt(q, k, v, a, b, dtype)
+    for _ in range(3):
+        again = G.grinqh_prompt_attention(q, k, v, a, b)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 def test_prompt_long():
     check_prompt(*prompt_case([1500, 20], [1500, 2500], 2, 1, 128, "bf16", 7), "bf16")
 

@@ -28,6 +28,10 @@
 // 128: that is what bounds the kernel there, and the exponentials, 8 cycles for a warp's
 // 32 of them or 2048 a round, at head_dim 64.
 //
+// Where there are few items for the SMs (a chunk after a long prefix), each item's keys are
+// cut into the same number of parts, items of their own; each writes its sums to the
+// workspace and a second kernel joins them in order.
+//
 // Keys past the sequence's end belong to another sequence and may hold anything: their
 // scores are masked, the O += P V steps of 16 keys past the last visible one are not
 // issued, and the at most 15 rows of V behind it are cleared in shared memory.
@@ -35,12 +39,13 @@
 #include "prompt_attention.cuh"
 #include "tmap.cuh"
 
-#include <type_traits>
+#include <algorithm>
 
 namespace grinqh {
 namespace {
 
 constexpr int kRows = 128;    // rows of a tile: tokens x query heads
+constexpr int kKeys = 128;    // keys of a block
 constexpr int kThreads = 384;
 constexpr float kSlack = 8.0f;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -53,12 +58,13 @@ struct PromptArgs {
   int total_q, total_k;
   int seqs, heads, kv_heads, group;  // group: query heads of a kv head
   int tokens;                        // of a tile: 128 / group
+  int parts;                         // of an item's keys
   float scale_log2;                  // softmax scale * log2(e)
+  float* sums;                       // [item][part][tile]{O[D / 4][row][4], {m, l}[row], token[row]}, for parts > 1
 };
 
 template <int D>
 struct Shape {
-  static constexpr int kKeys = 128;                      // of a block
   static constexpr int kAtoms = D / 64;                  // 64-channel (128-byte) columns of a tile or block
   static constexpr uint32_t kQAtom = kRows * 128;        // bytes of one
   static constexpr uint32_t kQBytes = kAtoms * kQAtom;
@@ -77,25 +83,36 @@ struct Item {
   int k0, m;      // first key row, keys of the sequence
   int token;      // first token of the tiles in the sequence
   int kv_head;    // < 0: no more items
+  int begin, end;  // the key blocks of this part
+  int index, part;
   __device__ __forceinline__ int first(int t, int tokens) const { return token + t * tokens; }
   // keys that the last token of tile t sees, and blocks of them
   __device__ __forceinline__ int keys(int t, int tokens) const {
     return max(0, min(m, m - n + min(n, first(t, tokens) + tokens)));
   }
-  template <int KEYS>
+  __device__ __forceinline__ int all_blocks(int t, int tokens) const {
+    return first(t, tokens) < n ? (keys(t, tokens) + kKeys - 1) / kKeys : 0;
+  }
+  // of them, those of this part
   __device__ __forceinline__ int blocks(int t, int tokens) const {
-    return first(t, tokens) < n ? (keys(t, tokens) + KEYS - 1) / KEYS : 0;
+    return max(0, min(all_blocks(t, tokens), end) - begin);
   }
 };
 
-// Finds token block `want` (of `tokens` each, counted from the last one) over all sequences; one warp.
-__device__ __forceinline__ Item find_item(const PromptArgs& a, int tokens, int64_t want, int kv_head) {
+// Finds item `at`, token blocks of `tokens` each being counted from the last one over all
+// sequences; one warp. order: the sequences by the keys they have, or null.
+__device__ __forceinline__ Item find_item(const PromptArgs& a, const int* order, int tokens, int at) {
   const int lane = threadIdx.x & 31;
-  Item it{0, 0, 0, 0, 0, -1};
+  Item it{0, 0, 0, 0, 0, -1, 0, 0, 0, 0};
+  if (at < 0) return it;
+  const int kv_head = at % a.kv_heads, part = at / a.kv_heads % a.parts;
+  int want = at / a.kv_heads / a.parts;
+  it.index = want * a.kv_heads + kv_head;
+  it.part = part;
   // sequences from the last to the first, 32 at a time, and their tokens from the last,
   // which see the most keys
   for (int top = a.seqs; top > 0; top -= 32) {
-    const int b = top - 1 - lane;
+    const int b = order && top - 1 - lane >= 0 ? order[top - 1 - lane] : top - 1 - lane;
     int q0 = 0, q1 = 0;
     if (b >= 0) {
       q0 = min(max(a.cu_q[b], 0), a.total_q);
@@ -113,13 +130,16 @@ __device__ __forceinline__ Item find_item(const PromptArgs& a, int tokens, int64
       const int src = __ffs(hit) - 1;
       const int before = __shfl_sync(0xffffffffu, upto - count, src);
       const int cnt = __shfl_sync(0xffffffffu, count, src);
-      const int bb = top - 1 - src;
+      const int bb = __shfl_sync(0xffffffffu, b, src);
       it.q0 = __shfl_sync(0xffffffffu, q0, src);
       it.n = __shfl_sync(0xffffffffu, q1, src) - it.q0;
-      it.token = (cnt - 1 - (int)(want - before)) * tokens;
+      it.token = (cnt - 1 - (want - before)) * tokens;
       it.k0 = min(max(a.cu_k[bb], 0), a.total_k);
       it.m = min(max(a.cu_k[bb + 1], it.k0), a.total_k) - it.k0;
       it.kv_head = kv_head;
+      const int all = max(it.all_blocks(0, tokens / 2), it.all_blocks(1, tokens / 2));
+      it.begin = (int)((int64_t)all * part / a.parts);
+      it.end = (int)((int64_t)all * (part + 1) / a.parts);
       return it;
     }
     want -= __shfl_sync(0xffffffffu, upto, 31);
@@ -138,13 +158,16 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// Sums of a tile of one part, in floats.
+__host__ __device__ constexpr int64_t sums_floats(int dim) { return (int64_t)kRows * (dim + 3); }
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
                                                                        const __grid_constant__ CUtensorMap tmap_k,
                                                                        const __grid_constant__ CUtensorMap tmap_v,
                                                                        const PromptArgs a) {
   using S = Shape<D>;
-  constexpr int kKeys = S::kKeys, ST = S::kStages;
+  constexpr int ST = S::kStages;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -166,6 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_full + 1);
   Item* s_item = reinterpret_cast<Item*>(tmem_slot + 2);  // [2]
   __shared__ __align__(16) uint32_t s_next[4];
+  __shared__ int s_order[32];
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == 9) {
@@ -204,16 +228,37 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   };
 
   // The softmax warps take the registers that the others do not need:
-  // 256 x 224 + 128 x 56 = 384 x 168, what the launch holds.
+  // 256 x 232 + 128 x 40 = 384 x 168, what the launch holds.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 8) {
       // ---------------------------------------------------------- items, TMA producer
       int stage = 0, round = 1, used = 0;  // ring stage and parity of its release; items so far
-      int64_t at = blockIdx.x;
+      // The next item is asked for when this one's last kAhead loads are left and looked up
+      // kFind before its end, so that neither is waited for (a few microseconds an item) and
+      // an SM that is behind still takes fewer.
+      constexpr int kAhead = 12, kFind = 4;
+      auto ask = [&] {
+        if (lane == 0) {
+          fence_proxy_async_smem();  // the last answer has been read
+          mbar_arrive_expect_tx(c_full, 16);
+          next_cta_ask(s_next, c_full);
+        }
+        __syncwarp();
+      };
+      const int* order = nullptr;
+      if (a.seqs <= 32) {  // few sequences: the longest start first
+        int keys = lane < a.seqs ? a.cu_k[lane + 1] - a.cu_k[lane] : 0, rank = 0;
+        for (int o = 0; o < a.seqs; ++o) {
+          const int other = __shfl_sync(0xffffffffu, keys, o);
+          rank += other < keys || (other == keys && o < lane);
+        }
+        if (lane < a.seqs) s_order[rank] = lane;
+        __syncwarp();
+        order = s_order;
+      }
+      Item it = find_item(a, order, 2 * tokens, (int)blockIdx.x);
       for (int k = 0;; ++k) {
-        Item it{0, 0, 0, 0, 0, -1};
-        if (at >= 0) it = find_item(a, 2 * tokens, at / a.kv_heads, (int)(at % a.kv_heads));
         if (k >= 2) mbar_wait_nocall(&i_empty[k & 1], ((k >> 1) - 1) & 1);
         if (lane == 0) {
           s_item[k & 1] = it;
@@ -221,8 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         }
         __syncwarp();
         if (it.kv_head < 0) break;
-        const int nb = max(it.blocks<kKeys>(0, tokens), it.blocks<kKeys>(1, tokens));
-        if (nb > 0) {
+        const int loads = 2 * max(it.blocks(0, tokens), it.blocks(1, tokens));
+        if (loads > 0) {
           if (used > 0) mbar_wait_nocall(q_empty, (used - 1) & 1);
           ++used;
           if (lane == 0) {
@@ -233,30 +278,34 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
                 tma_load_3d(s_q + t * S::kQBytes + c * S::kQAtom, &tmap_q, 64 * c, it.kv_head * a.group,
                             it.q0 + it.first(t, tokens), q_full);
           }
-          for (int n = 0; n < 2 * nb; ++n) {  // K of block 0, V of block 0, K of block 1, ...
-            mbar_wait_nocall(&empty[stage], round);
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&full[stage], S::kBytes);
-              for (int c = 0; c < S::kAtoms; ++c)
-                tma_load_3d(s_kv + stage * S::kBytes + c * S::kAtom, n & 1 ? &tmap_v : &tmap_k, 64 * c, it.kv_head,
-                            it.k0 + (n >> 1) * kKeys, &full[stage]);
-            }
-            __syncwarp();
-            if (++stage == ST) {
-              stage = 0;
-              round ^= 1;
-            }
+        }
+        Item following = it;
+        auto find = [&] {
+          const bool answered = mbar_wait_nocall(c_full, k & 1);
+          following = find_item(a, order, 2 * tokens, answered ? (int)next_cta_answer(s_next) : -1);
+        };
+        const int when_ask = max(0, loads - kAhead), when_find = max(0, loads - kFind);
+        for (int n = 0; n < loads; ++n) {  // K of block 0, V of block 0, K of block 1, ...
+          if (n == when_ask) ask();
+          if (n == when_find) find();
+          mbar_wait_nocall(&empty[stage], round);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&full[stage], S::kBytes);
+            for (int c = 0; c < S::kAtoms; ++c)
+              tma_load_3d(s_kv + stage * S::kBytes + c * S::kAtom, n & 1 ? &tmap_v : &tmap_k, 64 * c, it.kv_head,
+                          it.k0 + (it.begin + (n >> 1)) * kKeys, &full[stage]);
+          }
+          __syncwarp();
+          if (++stage == ST) {
+            stage = 0;
+            round ^= 1;
           }
         }
-        // the next item is asked for only now: an SM that is behind takes fewer
-        if (lane == 0) {
-          fence_proxy_async_smem();  // the last answer has been read
-          mbar_arrive_expect_tx(c_full, 16);
-          next_cta_ask(s_next, c_full);
+        if (loads == 0) {
+          ask();
+          find();
         }
-        const bool answered = mbar_wait_nocall(c_full, k & 1);
-        at = answered ? next_cta_answer(s_next) : -1;
-        __syncwarp();
+        it = following;
       }
     } else if (warp == 9) {
       // ---------------------------------------------------------- MMA issuer
@@ -319,9 +368,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       for (int k = 0;; ++k) {
         const Item it = item(k);
         if (uniform(it.kv_head) < 0) break;
-        const int nbt[2] = {uniform(it.blocks<kKeys>(0, tokens)), uniform(it.blocks<kKeys>(1, tokens))};
+        const int nbt[2] = {uniform(it.blocks(0, tokens)), uniform(it.blocks(1, tokens))};
         const int keys[2] = {uniform(it.keys(0, tokens)), uniform(it.keys(1, tokens))};
-        const int nb = max(nbt[0], nbt[1]), m = uniform(it.m);
+        const int nb = max(nbt[0], nbt[1]), begin = uniform(it.begin), m = uniform(it.m);
         if (nb == 0) continue;
         mbar_wait_nocall(q_full, used & 1);
         ++used;
@@ -333,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         if (nb == 1) commit(q_empty);
         for (int j = 0; j < nb; ++j) {
           const int vs = next();
-          const int left = m - j * kKeys;  // keys of the sequence from this block on
+          const int left = m - (begin + j) * kKeys;  // keys of the sequence from this block on
           if (left < kKeys && (left & 15)) {
             // rows of V behind the sequence's end in its last step of 16 keys
             for (int r = left + (lane >> 3); r < ((left + 15) & ~15); r += 4)
@@ -352,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
               if (no[t] > 0) mbar_wait_nocall(&o_empty[t], (no[t] - 1) & 1);
               ++no[t];
             }
-            outputs(t, vs, min(kKeys / 16, (keys[t] - j * kKeys + 15) / 16), j > 0);
+            outputs(t, vs, min(kKeys / 16, (keys[t] - (begin + j) * kKeys + 15) / 16), j > 0);
           }
           if (j + 1 < nb) commit(&empty[ks]);
           if (j + 2 == nb) commit(q_empty);
@@ -361,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ------------------------------------------------------------ softmax, epilogue
     const int t = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile
@@ -374,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
     for (int k = 0;; ++k) {
       const Item it = item(k);
       if (it.kv_head < 0) break;
-      const int nb = it.blocks<kKeys>(t, tokens);
+      const int nb = it.blocks(t, tokens);
       const int token = it.first(t, tokens) + r_token;         // of the sequence
       const int seen = min(it.m, it.m - it.n + token + 1);      // keys this row sees (<= 0: none)
       const int all_see = min(it.m, it.m - it.n + it.first(t, tokens) + 1);  // keys that every row sees
@@ -389,8 +438,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         tmem_ld_wait();
         tc_fence_before();
         mbar_arrive(s_empty);
-        if ((j + 1) * kKeys > all_see) {
-          const int lim = seen - j * kKeys;
+        if ((it.begin + j + 1) * kKeys > all_see) {
+          const int lim = seen - (it.begin + j) * kKeys;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -452,44 +501,141 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         mbar_arrive(&p_full[t]);
       }
       const float l = (l0.x + l0.y) + (l1.x + l1.y);
-      const bool in = token < it.n && r_token < tokens, none = m == -INFINITY && l == l;  // no score but -inf
+      const bool in = token < it.n && r_token < tokens;
       const int64_t at = (int64_t)(it.q0 + token) * a.heads + it.kv_head * a.group + r_head;
       T* out = static_cast<T*>(a.out) + at * D;
-      const float inv = 1.0f / l;
+      auto store = [&](int d, const float (&v)[8], float inv, bool none) {
+        uint32_t w[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = none ? 0u : pack2<T>(v[2 * x] * inv, v[2 * x + 1] * inv);
+        *reinterpret_cast<uint4*>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+      };
       if (nb > 0) {
         mbar_wait_nocall(&o_full[t], (ns - 1) & 1);
         tc_fence_after();
       }
+      const bool none = m == -INFINITY && l == l;  // no score but -inf
+      const float inv = 1.0f / l;
+      float* sums = a.sums + (((int64_t)it.index * a.parts + it.part) * 2 + t) * sums_floats(D);
+      // 32 channels of O at once: with more, the loop above loses registers
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int h = 0; h < D; h += 32) {
         uint32_t o[32];
         if (nb > 0) {
-          tmem_ld32(to + 32 * c, o);
+          tmem_ld32(to + h, o);
           tmem_ld_wait();
-          if (c == D / 32 - 1) {
+          if (h + 32 == D) {
             tc_fence_before();
             mbar_arrive(&o_empty[t]);
           }
         }
-        if (in) {
+        if (a.parts > 1) {
+          if (nb > 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
+            for (int d = 0; d < 32; d += 4)
+              __stcg(reinterpret_cast<uint4*>(sums) + (h + d) / 4 * kRows + r,
+                     make_uint4(o[d], o[d + 1], o[d + 2], o[d + 3]));
+          }
+        } else if (in) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-              w[x] = none ? 0u
-                          : pack2<T>(__uint_as_float(o[8 * i + 2 * x]) * inv, __uint_as_float(o[8 * i + 2 * x + 1]) * inv);
-            *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int d = 0; d < 32; d += 8) {
+            float v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = __uint_as_float(o[d + x]);
+            store(h + d, v, inv, none);
           }
         }
         __syncwarp();
       }
-      if (in) a.lse[at] = none ? -INFINITY : m * kLn2 + logf(l);
+      if (a.parts == 1) {
+        if (in) a.lse[at] = none ? -INFINITY : m * kLn2 + logf(l);
+        continue;
+      }
+      // a part of an item
+      __stcg(reinterpret_cast<float2*>(sums + kRows * D) + r, make_float2(nb > 0 ? m : -INFINITY, nb > 0 ? l : 0.f));
+      __stcg(reinterpret_cast<int*>(sums + kRows * (D + 2)) + r, in ? it.q0 + token : -1);
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 9) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Joins the parts of an item: blockIdx.x is item and tile, blockIdx.y 32 of the channels; a
+// thread takes a row.
+template <typename T, int D>
+__global__ void __launch_bounds__(kRows) join_kernel(const PromptArgs a) {
+  const int index = blockIdx.x >> 1, t = blockIdx.x & 1, r = threadIdx.x, d0 = 32 * blockIdx.y;
+  // how many items there are
+  int count = 0;
+  for (int b = threadIdx.x & 31; b < a.seqs; b += 32) {
+    const int q0 = min(max(a.cu_q[b], 0), a.total_q), q1 = min(max(a.cu_q[b + 1], q0), a.total_q);
+    count += (q1 - q0 + 2 * a.tokens - 1) / (2 * a.tokens);
+  }
+  if (index >= __reduce_add_sync(0xffffffffu, count) * a.kv_heads) return;
+  const float* sums = a.sums + ((int64_t)index * a.parts * 2 + t) * sums_floats(D);
+  const int token = __ldcg(reinterpret_cast<const int*>(sums + kRows * (D + 2)) + r);
+  if (token < 0) return;
+  float top = -INFINITY, all = 0.f, v[32];
+#pragma unroll
+  for (int d = 0; d < 32; ++d) v[d] = 0.f;
+#pragma unroll 2
+  for (int p = 0; p < a.parts; ++p, sums += 2 * sums_floats(D)) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(sums + kRows * D) + r);
+    float4 x[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) x[d] = __ldcg(reinterpret_cast<const float4*>(sums) + (d0 / 4 + d) * kRows + r);
+    if (ml.y == 0.f) continue;  // it saw nothing, and wrote no sums (a NaN counts)
+    const float now = fmaxf(top, ml.x);
+    const float f = now == -INFINITY ? 1.0f : exp2_fast(top - now), g = exp2_fast(ml.x - now);
+    top = now;
+    all = fmaf(ml.y, g, all * f);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      v[4 * d] = fmaf(x[d].x, g, v[4 * d] * f), v[4 * d + 1] = fmaf(x[d].y, g, v[4 * d + 1] * f);
+      v[4 * d + 2] = fmaf(x[d].z, g, v[4 * d + 2] * f), v[4 * d + 3] = fmaf(x[d].w, g, v[4 * d + 3] * f);
+    }
+  }
+  const bool none = top == -INFINITY && all == all;
+  const float inv = 1.0f / all;
+  const int64_t at = (int64_t)token * a.heads + index % a.kv_heads * a.group + r % a.group;
+  T* out = static_cast<T*>(a.out) + at * D + d0;
+#pragma unroll
+  for (int d = 0; d < 32; d += 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = none ? 0u : pack2<T>(v[d + 2 * i] * inv, v[d + 2 * i + 1] * inv);
+    *reinterpret_cast<uint4*>(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (d0 == 0) a.lse[at] = none ? -INFINITY : top * kLn2 + logf(all);
+}
+
+// Every sequence's tokens fill whole items but its last: at most this many.
+int64_t most_items(int64_t total_q, int64_t seqs, int tokens, int kv_heads) {
+  return std::min<int64_t>(total_q / (2 * tokens) + seqs, total_q) * kv_heads;
+}
+
+// Parts of an item's keys. The lengths are on the device, so this goes by what the host
+// knows. With two items per SM the large ones first balance well enough, and the sums of
+// parts (8 D bytes a row, written and read) would cost more than they save: 16384 tokens
+// x 8 heads, 514 items, lose 40 us. Below that, three parts' items per SM, of 4 blocks or more
+// on average: chunks of 2222 tokens over 17863 keys, 264 items, XXX us -> YYY.
+int parts_for(int64_t items, int64_t total_k, int64_t seqs, int sms) {
+  const int64_t blocks = total_k / std::max<int64_t>(seqs, 1) / kKeys;
+  if (items <= 0 || items >= 2 * sms || blocks < 8) return 1;
+  return (int)std::min<int64_t>({(3 * (int64_t)sms + items - 1) / items, blocks / 4, 16});
+}
+
+constexpr size_t kTicketRegion = 16 << 10;  // the workspace's start is kept zero for the linears' tickets
+
+int sm_count() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  return sms;
 }
 
 template <typename T, int D>
@@ -499,11 +645,13 @@ int launch(const PromptArgs& a, const CUtensorMap& q, const CUtensorMap& k, cons
   const cudaError_t e =
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<D>::kSmem);
   if (e != cudaSuccess) return set_error(GRINQH_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  // every sequence's tokens fill whole items but its last: at most this many
-  const int64_t items = std::min<int64_t>(a.total_q / (2 * a.tokens) + a.seqs, a.total_q) * a.kv_heads;
+  const int64_t items = most_items(a.total_q, a.seqs, a.tokens, a.kv_heads) * a.parts;
   GRINQH_REQUIRE(items < (1LL << 31), "too many row blocks (%lld)", (long long)items);
   kern<<<(unsigned)items, kThreads, Shape<D>::kSmem, st>>>(q, k, v, a);
-  return check_launch("prompt_attention");
+  GRINQH_RETURN_IF(check_launch("prompt_attention"));
+  if (a.parts == 1) return GRINQH_OK;
+  join_kernel<T, D><<<dim3((unsigned)(items / a.parts * 2), D / 32), kRows, 0, st>>>(a);
+  return check_launch("prompt_attention (join)");
 }
 
 }  // namespace
@@ -519,12 +667,23 @@ unsigned take_prompt_timeouts() {
 
 using namespace grinqh;
 
+extern "C" size_t grinqh_prompt_attention_workspace_size(int64_t total_q, int64_t total_k, int num_seqs, int num_heads,
+                                                         int num_kv_heads, int head_dim) {
+  if (total_q <= 0 || num_seqs <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      num_heads / num_kv_heads > kRows || num_heads <= 0)
+    return 0;
+  const int64_t items = most_items(total_q, num_seqs, kRows / (num_heads / num_kv_heads), num_kv_heads);
+  const int parts = parts_for(items, total_k, num_seqs, sm_count());
+  return parts == 1 ? 0 : kTicketRegion + (size_t)items * parts * 2 * sums_floats(head_dim) * sizeof(float);
+}
+
 extern "C" int grinqh_prompt_attention(const void* q, const void* k, const void* v, int dtype, int64_t total_q,
                                        int64_t total_k, int num_seqs, int num_heads, int num_kv_heads, int head_dim,
                                        int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
                                        int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
                                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, float softmax_scale,
-                                       void* out, float* lse, grinqh_stream_t stream) {
+                                       void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                       grinqh_stream_t stream) {
   GRINQH_RETURN_IF(check_device());
   GRINQH_REQUIRE(dtype == GRINQH_BF16 || dtype == GRINQH_F16, "dtype must be GRINQH_BF16 or GRINQH_F16");
   if (head_dim != 64 && head_dim != 128)
@@ -543,17 +702,37 @@ extern "C" int grinqh_prompt_attention(const void* q, const void* k, const void*
   const int group = num_heads / num_kv_heads;
   if (group > kRows)
     return set_error(GRINQH_ERR_UNSUPPORTED, "at most %d query heads per kv head (got %d)", kRows, group);
-  const PromptArgs a{cu_seqlens_q, cu_seqlens_k, out,          lse,   (int)total_q,  (int)total_k,
-                     num_seqs,     num_heads,    num_kv_heads, group, kRows / group, softmax_scale * 1.4426950408889634f};
+  PromptArgs a{};
+  a.cu_q = cu_seqlens_q;
+  a.cu_k = cu_seqlens_k;
+  a.out = out;
+  a.lse = lse;
+  a.total_q = (int)total_q;
+  a.total_k = (int)total_k;
+  a.seqs = num_seqs;
+  a.heads = num_heads;
+  a.kv_heads = num_kv_heads;
+  a.group = group;
+  a.tokens = kRows / group;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  const int64_t items = most_items(total_q, num_seqs, a.tokens, num_kv_heads);
+  a.parts = parts_for(items, total_k, num_seqs, sm_count());
+  if (a.parts > 1) {
+    const size_t need = grinqh_prompt_attention_workspace_size(total_q, total_k, num_seqs, num_heads, num_kv_heads,
+                                                               head_dim);
+    if (!workspace || workspace_bytes < need)
+      return set_error(GRINQH_ERR_WORKSPACE, "workspace of %zu bytes required (got %zu)", need, workspace_bytes);
+    GRINQH_REQUIRE(aligned(workspace, 256), "workspace must be 256-byte aligned");
+    a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + kTicketRegion);
+  }
   const bool bf16 = dtype == GRINQH_BF16;
-  const uint32_t box = head_dim == 128 ? Shape<128>::kKeys : Shape<64>::kKeys;
   CUtensorMap tq, tk, tv;
   GRINQH_RETURN_IF(tmap_heads(&tq, bf16, q, total_q, num_heads, head_dim, q_token_stride, q_head_stride, group,
                               a.tokens, "q"));
   if (total_k > 0) {
-    GRINQH_RETURN_IF(tmap_heads(&tk, bf16, k, total_k, num_kv_heads, head_dim, k_token_stride, k_head_stride, 1, box,
+    GRINQH_RETURN_IF(tmap_heads(&tk, bf16, k, total_k, num_kv_heads, head_dim, k_token_stride, k_head_stride, 1, kKeys,
                                 "k"));
-    GRINQH_RETURN_IF(tmap_heads(&tv, bf16, v, total_k, num_kv_heads, head_dim, v_token_stride, v_head_stride, 1, box,
+    GRINQH_RETURN_IF(tmap_heads(&tv, bf16, v, total_k, num_kv_heads, head_dim, v_token_stride, v_head_stride, 1, kKeys,
                                 "v"));
   } else {
     tk = tv = tq;  // never read: no row sees a key

@@ -576,11 +576,18 @@ std::tuple<at::Tensor, at::Tensor> prompt_attention(const at::Tensor& q, const a
   at::Tensor out = at::empty(q.sizes(), q.options());
   at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
   if (out.numel() == 0) return {out, lse};
+  const cudaStream_t stream = cur_stream(q);
+  const size_t bytes = grinqh_prompt_attention_workspace_size(q.size(0), k.size(0), (int)(cq.size(0) - 1), (int)q.size(1),
+                                                              (int)k.size(1), (int)q.size(2));
+  at::Tensor ws;
+  bool zeroed = false;
+  if (bytes) ws = stream_workspace(q, bytes, stream, &zeroed);
   check_ok(grinqh_prompt_attention(qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), dt, q.size(0), k.size(0),
                                    (int)(cq.size(0) - 1), (int)q.size(1), (int)k.size(1), (int)q.size(2), qc.stride(0),
                                    qc.stride(1), kc.stride(0), kc.stride(1), vc.stride(0), vc.stride(1),
                                    cq.data_ptr<int32_t>(), ck.data_ptr<int32_t>(), (float)softmax_scale,
-                                   out.data_ptr(), lse.data_ptr<float>(), cur_stream(q)),
+                                   out.data_ptr(), lse.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr,
+                                   bytes ? static_cast<size_t>(ws.numel()) : 0, stream),
            "prompt_attention");
   return {out, lse};
 }

@@ -64,7 +64,8 @@ SIGNATURES = {
     "grinqh_kv4_attention": (_int, [_ptr, _int, _i64, _int, _int, _int, _int, _int, _i64, _i64, _i64, _ptr, _i64, _int,
                                     _ptr, _i64, _i64, _ptr, ctypes.c_float, _ptr, _ptr, _ptr, _size, _int, _ptr]),
     "grinqh_prompt_attention": (_int, [_ptr, _ptr, _ptr, _int, _i64, _i64, _int, _int, _int, _int, _i64, _i64, _i64,
-                                       _i64, _i64, _i64, _ptr, _ptr, ctypes.c_float, _ptr, _ptr, _ptr]),
+                                       _i64, _i64, _i64, _ptr, _ptr, ctypes.c_float, _ptr, _ptr, _ptr, _size, _ptr]),
+    "grinqh_prompt_attention_workspace_size": (_size, [_i64, _i64, _int, _int, _int, _int]),
     "grinqh_gemv_noalloc": (_int, [_ptr, _int, _i64, _ptr, _ptr, _ptr, _int, _int, _i64, _fptr, _ptr, _ptr]),
 }
 
