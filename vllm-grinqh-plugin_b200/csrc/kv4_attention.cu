@@ -28,6 +28,7 @@
 // each writes its sums to the workspace and the last one to arrive joins them in order.
 #include "kv4.cuh"
 #include "kv4_attention.cuh"
+#include "launch.cuh"
 #include "ptx.cuh"
 
 #include <algorithm>
@@ -202,6 +203,10 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
     fence_mbar_init();
     s_left[warp].flags = 0;
   }
+
+  // the next kernel's set-up may overlap this one, as this one's did its predecessor
+  allow_dependent_grid();
+  wait_prior_grid();
 
   // ---------------------------------------------------------------- the CTA's runs
   if (warp == NW) {
@@ -844,16 +849,6 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return 148;
-  }
-  return sms;
-}
-
 constexpr size_t kTicketRegion = 16 << 10;  // where the linears keep theirs: all zero between calls
 static_assert(kTicketRegion >= 4 * 1024, "a ticket per CTA, one CTA per SM");
 
@@ -863,10 +858,9 @@ template <typename T, int D, int GS, int NT>
 int launch(const Kv4AttnArgs& a, int sms, cudaStream_t st) {
   using P = Plan<D, GS, NT>;
   auto kern = kv4_attention_kernel<T, D, GS, NT>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::kSmem);
-  if (e != cudaSuccess) return set_error(GRINQH_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  kern<<<(unsigned)sms, P::kThreads, P::kSmem, st>>>(a);
-  return check_launch("kv4_attention");
+  static std::atomic<uint64_t> ready{0};
+  GRINQH_RETURN_IF(allow_smem(reinterpret_cast<const void*>(kern), ready, P::kSmem));
+  return launch_dependent(kern, dim3((unsigned)sms), P::kThreads, P::kSmem, st, "kv4_attention", a);
 }
 
 }  // namespace

@@ -35,6 +35,7 @@
 // Keys past the sequence's end belong to another sequence and may hold anything: their
 // scores are masked, the O += P V steps of 16 keys past the last visible one are not
 // issued, and the at most 15 rows of V behind it are cleared in shared memory.
+#include "launch.cuh"
 #include "ptx.cuh"
 #include "prompt_attention.cuh"
 #include "tmap.cuh"
@@ -216,6 +217,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // the next kernel's set-up may overlap this one, as this one's did its predecessor
+  allow_dependent_grid();
+  wait_prior_grid();
   const uint32_t tmem = *tmem_slot;
   const int tokens = a.tokens;
   // the k-th item of this CTA, for every warp but the one that finds it
@@ -566,6 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
 template <typename T, int D>
 __global__ void __launch_bounds__(kRows) join_kernel(const PromptArgs a) {
   const int index = blockIdx.x >> 1, t = blockIdx.x & 1, r = threadIdx.x, d0 = 32 * blockIdx.y;
+  allow_dependent_grid();
+  wait_prior_grid();
   // how many items there are
   int count = 0;
   for (int b = threadIdx.x & 31; b < a.seqs; b += 32) {
@@ -628,30 +634,19 @@ int parts_for(int64_t items, int64_t total_k, int64_t seqs, int sms) {
 
 constexpr size_t kTicketRegion = 16 << 10;  // the workspace's start is kept zero for the linears' tickets
 
-int sm_count() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return 148;
-  }
-  return sms;
-}
-
 template <typename T, int D>
 int launch(const PromptArgs& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v,
            cudaStream_t st) {
   auto kern = prompt_attention_kernel<T, D>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<D>::kSmem);
-  if (e != cudaSuccess) return set_error(GRINQH_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> ready{0};
+  GRINQH_RETURN_IF(allow_smem(reinterpret_cast<const void*>(kern), ready, Shape<D>::kSmem));
   const int64_t items = most_items(a.total_q, a.seqs, a.tokens, a.kv_heads) * a.parts;
   GRINQH_REQUIRE(items < (1LL << 31), "too many row blocks (%lld)", (long long)items);
-  kern<<<(unsigned)items, kThreads, Shape<D>::kSmem, st>>>(q, k, v, a);
-  GRINQH_RETURN_IF(check_launch("prompt_attention"));
+  GRINQH_RETURN_IF(launch_dependent(kern, dim3((unsigned)items), kThreads, Shape<D>::kSmem, st, "prompt_attention", q,
+                                    k, v, a));
   if (a.parts == 1) return GRINQH_OK;
-  join_kernel<T, D><<<dim3((unsigned)(items / a.parts * 2), D / 32), kRows, 0, st>>>(a);
-  return check_launch("prompt_attention (join)");
+  return launch_dependent(join_kernel<T, D>, dim3((unsigned)(items / a.parts * 2), D / 32), kRows, 0, st,
+                          "prompt_attention (join)", a);
 }
 
 }  // namespace
