@@ -15,6 +15,7 @@ namespace grinqh {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kUnits = 2;  // tokens that a thread of the gather takes
 
 template <typename T> struct Pair;
 template <> struct Pair<__nv_bfloat16> {
@@ -62,26 +63,33 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& raw, uint32_t& params
   }
   const T zero = __hmin_nan(lo.x, lo.y), top = __hmax_nan(hi.x, hi.y);
   const float z = Act<T>::to_f(zero);
-  const T scale_t = Act<T>::from_f((Act<T>::to_f(top) - z) / 15.0f);
+  float step = (Act<T>::to_f(top) - z) / 15.0f;
+  step += step - step;  // an infinite one becomes NaN: so does every value of the group
+  const T scale_t = Act<T>::from_f(step);
   const float scale = Act<T>::to_f(scale_t);
   const float inv = scale >= 1.17549435e-38f ? 1.0f / scale : 0.0f;  // a smaller scale's inverse overflows
   T2 both;
   both.x = scale_t;
   both.y = zero;
   params = *reinterpret_cast<uint32_t*>(&both);
-  uint32_t codes = 0;
+  // x >= zero, so a code is rint(min(q, 15)): rounded by adding 1.5 2^23 and collected as
+  // the digits of a number to base 16, four at a time, which fp32 holds exactly. (One
+  // conversion to an integer per code would take the special function units 16 x 8 cycles
+  // a warp.) A NaN becomes 15.
+  constexpr float kRound = 12582912.0f;
+  float digits[2] = {kRound, kRound};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = Pair<T>::to_f(x[i]);
-    const float a = fminf(fmaxf((f.x - z) * inv, 0.0f), 15.0f), b = fminf(fmaxf((f.y - z) * inv, 0.0f), 15.0f);
-    codes |= (uint32_t)__float2int_rn(a) << (8 * i);
-    codes |= (uint32_t)__float2int_rn(b) << (8 * i + 4);
+    const float a = fminf((f.x - z) * inv, 15.0f), b = fminf((f.y - z) * inv, 15.0f);
+    digits[i / 2] = fmaf((a + kRound) - kRound, i % 2 ? 256.0f : 1.0f, digits[i / 2]);
+    digits[i / 2] = fmaf((b + kRound) - kRound, i % 2 ? 4096.0f : 16.0f, digits[i / 2]);
   }
-  return codes;
+  return __byte_perm(__float_as_uint(digits[0]), __float_as_uint(digits[1]), 0x5410u);
 }
 
-// One lane per 8 channels of a token and head; the lanes of tokens 2 p and 2 p + 1 are
-// neighbours, so that the pair's V words are written whole where both tokens lie in one
+// One lane per 8 channels of a token and head (blockIdx.y); the lanes of tokens 2 p and
+// 2 p + 1 are neighbours, so that the pair's V words are written whole where both tokens lie in one
 // pair row of the cache (else each token writes its 16-bit halves).
 template <typename T, int D, int GS>
 __global__ void __launch_bounds__(kThreads) append_kernel(const T* __restrict__ k, const T* __restrict__ v,
@@ -89,18 +97,15 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const T* __restrict__ 
                                                           int64_t v_head, CacheArgs a) {
   using L = Kv4<D, GS>;
   constexpr int kLanes = D / 8;
-  const int64_t tid = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int l = (int)(tid % kLanes);
-  const int odd = (int)(tid / kLanes) & 1;
-  const int64_t unit = tid / (2 * kLanes);
-  const int h = (int)(unit % a.kv_heads);
-  const int64_t i = 2 * (unit / a.kv_heads) + odd;
+  const int l = threadIdx.x % kLanes, odd = threadIdx.x / kLanes & 1, h = blockIdx.y;
+  const int64_t i = 2 * ((int64_t)blockIdx.x * (kThreads / (2 * kLanes)) + threadIdx.x / (2 * kLanes)) + odd;
   const bool in = i < a.tokens;
   int64_t slot = in ? a.slots[i] : -1;
   if (slot < 0 || slot >= a.capacity) slot = -1;
   const uint4 zero4 = make_uint4(0u, 0u, 0u, 0u);
-  const uint4 kr = slot >= 0 ? *reinterpret_cast<const uint4*>(k + i * k_token + h * k_head + 8 * l) : zero4;
-  const uint4 vr = slot >= 0 ? *reinterpret_cast<const uint4*>(v + i * v_token + h * v_head + 8 * l) : zero4;
+  // (not waiting for the slot)
+  const uint4 kr = in ? *reinterpret_cast<const uint4*>(k + i * k_token + h * k_head + 8 * l) : zero4;
+  const uint4 vr = in ? *reinterpret_cast<const uint4*>(v + i * v_token + h * v_head + 8 * l) : zero4;
   uint32_t kp, vp;
   const uint32_t kc = quantize8<T, GS>(kr, kp);
   const uint32_t vc = quantize8<T, GS>(vr, vp);
@@ -143,29 +148,46 @@ __device__ __forceinline__ uint4 values8(uint32_t codes, uint32_t params) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// One lane per 8 channels of a token and head.
+// One lane per 8 channels of a token and head (blockIdx.y), the lanes of tokens 2 p and
+// 2 p + 1 side by side: where they are a pair in the cache too, both read the same words of
+// V. A thread takes kUnits pairs of tokens, for more loads in flight behind the slots'.
 template <typename T, int D, int GS>
 __global__ void __launch_bounds__(kThreads) gather_kernel(CacheArgs a, T* __restrict__ k, T* __restrict__ v) {
   using L = Kv4<D, GS>;
   constexpr int kLanes = D / 8;
-  const int64_t tid = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int d = 8 * (int)(tid % kLanes);
-  const int64_t row = tid / kLanes;  // token * kv_heads + head
-  const int64_t i = row / a.kv_heads;
-  if (i >= a.tokens) return;
-  const int64_t slot = a.slots[i];
-  uint4 kv = make_uint4(0u, 0u, 0u, 0u), vv = kv;
-  if (slot >= 0 && slot < a.capacity) {
-    const int token = (int)(slot & 15);
-    const uint8_t* rec = a.cache + record_at<L::kRecord>(a, slot, (int)(row - i * a.kv_heads));
-    const uint32_t kc = reinterpret_cast<const uint32_t*>(rec + token * (D / 2))[L::k_word(d)];
-    const uint16_t* vrow = reinterpret_cast<const uint16_t*>(rec + L::kV + (token >> 1) * D) + (token & 1);
-    const uint32_t vc = vrow[2 * L::v_word(token >> 1, d)] | ((uint32_t)vrow[2 * L::v_word(token >> 1, d + 4)] << 16);
-    kv = values8<T>(kc, reinterpret_cast<const uint32_t*>(rec + L::kKParams)[token * L::NG + d / GS]);
-    vv = values8<T>(vc, reinterpret_cast<const uint32_t*>(rec + L::kVParams)[token * L::NG + d / GS]);
+  constexpr int kPairs = kThreads / (2 * kLanes);  // of a block at a time
+  const int d = 8 * (threadIdx.x % kLanes), h = blockIdx.y;
+  const int64_t first = 2 * ((int64_t)blockIdx.x * kUnits * kPairs + threadIdx.x / (2 * kLanes)) +
+                        (threadIdx.x / kLanes & 1);
+  int64_t slot[kUnits];
+  uint32_t kc[kUnits], v0[kUnits], v1[kUnits], kp[kUnits], vp[kUnits];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int64_t i = first + 2 * kPairs * u;
+    slot[u] = i < a.tokens ? a.slots[i] : -1;
+    if (slot[u] >= a.capacity) slot[u] = -1;
   }
-  *reinterpret_cast<uint4*>(k + row * D + d) = kv;
-  *reinterpret_cast<uint4*>(v + row * D + d) = vv;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    kc[u] = v0[u] = v1[u] = kp[u] = vp[u] = 0u;
+    if (slot[u] < 0) continue;
+    const int token = (int)(slot[u] & 15), pair = token >> 1;
+    const uint8_t* rec = a.cache + record_at<L::kRecord>(a, slot[u], h);
+    kc[u] = __ldg(reinterpret_cast<const uint32_t*>(rec + token * (D / 2)) + L::k_word(d));
+    v0[u] = __ldg(reinterpret_cast<const uint32_t*>(rec + L::kV + pair * D) + L::v_word(pair, d));
+    v1[u] = __ldg(reinterpret_cast<const uint32_t*>(rec + L::kV + pair * D) + L::v_word(pair, d + 4));
+    kp[u] = __ldg(reinterpret_cast<const uint32_t*>(rec + L::kKParams) + token * L::NG + d / GS);
+    vp[u] = __ldg(reinterpret_cast<const uint32_t*>(rec + L::kVParams) + token * L::NG + d / GS);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const int64_t i = first + 2 * kPairs * u;
+    if (i >= a.tokens) continue;
+    const int64_t at = (i * a.kv_heads + h) * D + d;
+    const uint32_t vc = __byte_perm(v0[u], v1[u], slot[u] & 1 ? 0x7632u : 0x5410u);
+    __stcs(reinterpret_cast<uint4*>(k + at), values8<T>(kc[u], kp[u]));
+    __stcs(reinterpret_cast<uint4*>(v + at), values8<T>(vc, vp[u]));
+  }
 }
 
 }  // namespace
@@ -189,17 +211,17 @@ extern "C" int grinqh_kv4_append(const void* k, const void* v, int dtype, int64_
                      v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
                  "k, v and their strides must be 16-byte aligned");
   const CacheArgs a{cache, slots, tokens, num_pages * page_size, num_kv_heads, (uint32_t)(page_size / kTile)};
-  const int64_t threads = (tokens + 1) / 2 * num_kv_heads * 2 * (head_dim / 8);
-  const int64_t grid = (threads + kThreads - 1) / kThreads;
-  GRINQH_REQUIRE(grid < (1LL << 31), "tokens out of range (%lld)", (long long)tokens);
+  const int pairs = kThreads / (2 * (head_dim / 8));  // of a block
+  const int64_t blocks = ((tokens + 1) / 2 + pairs - 1) / pairs;
+  const dim3 grid((unsigned)blocks, (unsigned)num_kv_heads);
   return kv4_dispatch(head_dim, group_size, [&](auto layout) {
     using L = decltype(layout);
     if (dtype == GRINQH_BF16)
-      append_kernel<__nv_bfloat16, L::kDim, L::kGroup><<<(unsigned)grid, kThreads, 0, stream>>>(
+      append_kernel<__nv_bfloat16, L::kDim, L::kGroup><<<grid, kThreads, 0, stream>>>(
           static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), k_token_stride, k_head_stride,
           v_token_stride, v_head_stride, a);
     else
-      append_kernel<__half, L::kDim, L::kGroup><<<(unsigned)grid, kThreads, 0, stream>>>(
+      append_kernel<__half, L::kDim, L::kGroup><<<grid, kThreads, 0, stream>>>(
           static_cast<const __half*>(k), static_cast<const __half*>(v), k_token_stride, k_head_stride, v_token_stride,
           v_head_stride, a);
     return check_launch("kv4_append");
@@ -218,15 +240,16 @@ extern "C" int grinqh_kv4_gather(const uint8_t* cache, int dtype, int64_t num_pa
   GRINQH_REQUIRE(aligned(k, 16) && aligned(v, 16), "k and v must be 16-byte aligned");
   const CacheArgs a{const_cast<uint8_t*>(cache), slots,        tokens,
                     num_pages * page_size,       num_kv_heads, (uint32_t)(page_size / kTile)};
-  const int64_t grid = (tokens * num_kv_heads * (head_dim / 8) + kThreads - 1) / kThreads;
-  GRINQH_REQUIRE(grid < (1LL << 31), "tokens out of range (%lld)", (long long)tokens);
+  const int pairs = kUnits * (kThreads / (2 * (head_dim / 8)));  // of a block
+  const int64_t blocks = ((tokens + 1) / 2 + pairs - 1) / pairs;
+  const dim3 grid((unsigned)blocks, (unsigned)num_kv_heads);
   return kv4_dispatch(head_dim, group_size, [&](auto layout) {
     using L = decltype(layout);
     if (dtype == GRINQH_BF16)
-      gather_kernel<__nv_bfloat16, L::kDim, L::kGroup><<<(unsigned)grid, kThreads, 0, stream>>>(
+      gather_kernel<__nv_bfloat16, L::kDim, L::kGroup><<<grid, kThreads, 0, stream>>>(
           a, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
     else
-      gather_kernel<__half, L::kDim, L::kGroup><<<(unsigned)grid, kThreads, 0, stream>>>(a, static_cast<__half*>(k),
+      gather_kernel<__half, L::kDim, L::kGroup><<<grid, kThreads, 0, stream>>>(a, static_cast<__half*>(k),
                                                                              static_cast<__half*>(v));
     return check_launch("kv4_gather");
   });

@@ -60,6 +60,7 @@ struct PromptArgs {
   int seqs, heads, kv_heads, group;  // group: query heads of a kv head
   int tokens;                        // of a tile: 128 / group
   int parts;                         // of an item's keys
+  int more;                          // whether there are more items than SMs
   float scale_log2;                  // softmax scale * log2(e)
   float* sums;                       // [item][part][tile]{O[D / 4][row][4], {m, l}[row], token[row]}, for parts > 1
 };
@@ -100,9 +101,39 @@ struct Item {
   }
 };
 
+// A sequence's rows, cut to the tensors.
+struct Rows {
+  int q0, n, k0, m;
+};
+
+__device__ __forceinline__ Rows rows_of(const PromptArgs& a, int b) {
+  const int q0 = min(max(a.cu_q[b], 0), a.total_q), k0 = min(max(a.cu_k[b], 0), a.total_k);
+  return {q0, min(max(a.cu_q[b + 1], q0), a.total_q) - q0, k0, min(max(a.cu_k[b + 1], k0), a.total_k) - k0};
+}
+
+// The sequences if there are at most 32, one a lane, those with the most keys last.
+__device__ __forceinline__ Rows sorted_rows(const PromptArgs& a) {
+  const int lane = threadIdx.x & 31;
+  Rows mine{0, 0, 0, 0};
+  if (lane < a.seqs) mine = rows_of(a, lane);
+  int rank = lane;
+  if (a.seqs > 1) {
+    rank = lane < a.seqs ? 0 : lane;
+    for (int o = 0; o < a.seqs; ++o) {
+      const int other = __shfl_sync(0xffffffffu, mine.m, o);
+      if (lane < a.seqs) rank += other < mine.m || (other == mine.m && o < lane);
+    }
+  }
+  int from = lane;
+  for (int o = 0; o < a.seqs; ++o)
+    if (__shfl_sync(0xffffffffu, rank, o) == lane) from = o;
+  return {__shfl_sync(0xffffffffu, mine.q0, from), __shfl_sync(0xffffffffu, mine.n, from),
+          __shfl_sync(0xffffffffu, mine.k0, from), __shfl_sync(0xffffffffu, mine.m, from)};
+}
+
 // Finds item `at`, token blocks of `tokens` each being counted from the last one over all
-// sequences; one warp. order: the sequences by the keys they have, or null.
-__device__ __forceinline__ Item find_item(const PromptArgs& a, const int* order, int tokens, int at) {
+// sequences; one warp. few: the sequences if there are at most 32.
+__device__ __forceinline__ Item find_item(const PromptArgs& a, const Rows& few, int tokens, int at) {
   const int lane = threadIdx.x & 31;
   Item it{0, 0, 0, 0, 0, -1, 0, 0, 0, 0};
   if (at < 0) return it;
@@ -113,13 +144,16 @@ __device__ __forceinline__ Item find_item(const PromptArgs& a, const int* order,
   // sequences from the last to the first, 32 at a time, and their tokens from the last,
   // which see the most keys
   for (int top = a.seqs; top > 0; top -= 32) {
-    const int b = order && top - 1 - lane >= 0 ? order[top - 1 - lane] : top - 1 - lane;
-    int q0 = 0, q1 = 0;
-    if (b >= 0) {
-      q0 = min(max(a.cu_q[b], 0), a.total_q);
-      q1 = min(max(a.cu_q[b + 1], q0), a.total_q);
+    const int b = top - 1 - lane;
+    Rows rows;
+    if (a.seqs <= 32) {
+      const int from = max(b, 0);
+      rows = {__shfl_sync(0xffffffffu, few.q0, from), __shfl_sync(0xffffffffu, few.n, from),
+              __shfl_sync(0xffffffffu, few.k0, from), __shfl_sync(0xffffffffu, few.m, from)};
+    } else if (b >= 0) {
+      rows = rows_of(a, b);
     }
-    const int count = (q1 - q0 + tokens - 1) / tokens;
+    const int count = b >= 0 ? (rows.n + tokens - 1) / tokens : 0;
     int upto = count;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -131,12 +165,11 @@ __device__ __forceinline__ Item find_item(const PromptArgs& a, const int* order,
       const int src = __ffs(hit) - 1;
       const int before = __shfl_sync(0xffffffffu, upto - count, src);
       const int cnt = __shfl_sync(0xffffffffu, count, src);
-      const int bb = __shfl_sync(0xffffffffu, b, src);
-      it.q0 = __shfl_sync(0xffffffffu, q0, src);
-      it.n = __shfl_sync(0xffffffffu, q1, src) - it.q0;
+      it.q0 = __shfl_sync(0xffffffffu, rows.q0, src);
+      it.n = __shfl_sync(0xffffffffu, rows.n, src);
+      it.k0 = __shfl_sync(0xffffffffu, rows.k0, src);
+      it.m = __shfl_sync(0xffffffffu, rows.m, src);
       it.token = (cnt - 1 - (want - before)) * tokens;
-      it.k0 = min(max(a.cu_k[bb], 0), a.total_k);
-      it.m = min(max(a.cu_k[bb + 1], it.k0), a.total_k) - it.k0;
       it.kv_head = kv_head;
       const int all = max(it.all_blocks(0, tokens / 2), it.all_blocks(1, tokens / 2));
       it.begin = (int)((int64_t)all * part / a.parts);
@@ -190,7 +223,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_full + 1);
   Item* s_item = reinterpret_cast<Item*>(tmem_slot + 2);  // [2]
   __shared__ __align__(16) uint32_t s_next[4];
-  __shared__ int s_order[32];
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == 9) {
@@ -243,25 +275,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       // an SM that is behind still takes fewer.
       constexpr int kAhead = 12, kFind = 4;
       auto ask = [&] {
-        if (lane == 0) {
+        if (lane == 0 && a.more) {
           fence_proxy_async_smem();  // the last answer has been read
           mbar_arrive_expect_tx(c_full, 16);
           next_cta_ask(s_next, c_full);
         }
         __syncwarp();
       };
-      const int* order = nullptr;
-      if (a.seqs <= 32) {  // few sequences: the longest start first
-        int keys = lane < a.seqs ? a.cu_k[lane + 1] - a.cu_k[lane] : 0, rank = 0;
-        for (int o = 0; o < a.seqs; ++o) {
-          const int other = __shfl_sync(0xffffffffu, keys, o);
-          rank += other < keys || (other == keys && o < lane);
-        }
-        if (lane < a.seqs) s_order[rank] = lane;
-        __syncwarp();
-        order = s_order;
-      }
-      Item it = find_item(a, order, 2 * tokens, (int)blockIdx.x);
+      const Rows few = a.seqs <= 32 ? sorted_rows(a) : Rows{0, 0, 0, 0};  // the longest start first
+      Item it = find_item(a, few, 2 * tokens, (int)blockIdx.x);
       for (int k = 0;; ++k) {
         if (k >= 2) mbar_wait_nocall(&i_empty[k & 1], ((k >> 1) - 1) & 1);
         if (lane == 0) {
@@ -285,8 +307,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         }
         Item following = it;
         auto find = [&] {
-          const bool answered = mbar_wait_nocall(c_full, k & 1);
-          following = find_item(a, order, 2 * tokens, answered ? (int)next_cta_answer(s_next) : -1);
+          const bool answered = a.more && mbar_wait_nocall(c_full, k & 1);
+          following = find_item(a, few, 2 * tokens, answered ? (int)next_cta_answer(s_next) : -1);
         };
         const int when_ask = max(0, loads - kAhead), when_find = max(0, loads - kFind);
         for (int n = 0; n < loads; ++n) {  // K of block 0, V of block 0, K of block 1, ...
@@ -712,6 +734,7 @@ extern "C" int grinqh_prompt_attention(const void* q, const void* k, const void*
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   const int64_t items = most_items(total_q, num_seqs, a.tokens, num_kv_heads);
   a.parts = parts_for(items, total_k, num_seqs, sm_count());
+  a.more = items * a.parts > sm_count();
   if (a.parts > 1) {
     const size_t need = grinqh_prompt_attention_workspace_size(total_q, total_k, num_seqs, num_heads, num_kv_heads,
                                                                head_dim);
