@@ -761,27 +761,41 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
   // leaves open; a chain takes the heads of the warps behind it while they go through.
   // A thread takes 4 channels of a row of a chain.
   const int all = a.fresh * a.group;
+  // four warps a chain, as many chains at a time as there are
+  constexpr int kGroups = (NW + 1) / 4;
+  const bool is = lane <= NW && (s_left[max(lane - 1, 0)].flags & (lane == 0 ? kHead : kTail));
+  uint32_t chains = __ballot_sync(kFull, is);
+  for (int k = warp / 4; k > 0; --k) chains &= chains - 1u;
 #pragma unroll 1
-  for (int chain = 0; chain <= NW; ++chain) {
+  while (chains != 0u) {
+    const int chain = __ffs(chains) - 1;
+    for (int k = 0; k < kGroups; ++k) chains &= chains - 1u;
     const Left& first = s_left[max(chain - 1, 0)];
-    if (!(first.flags & (chain == 0 ? kHead : kTail))) continue;
     const Piece piece = chain == 0 ? first.head : first.tail;
     const int kv_head = piece.h / a.parts, row0 = (piece.h - kv_head * a.parts) * P::kRows;
     const int w0 = max(chain - 1, 0);
-    int w1 = w0;  // the chain's last warp
-    bool open = chain > 0 || (first.flags & kThrough);
-    while (open && w1 + 1 < NW) open = s_left[++w1].flags & kThrough;
-    for (int i = threadIdx.x; i < min(all - row0, P::kRows) * (D / 4); i += P::kThreads) {
+    // the chain's last warp: the first behind it whose head does not go through
+    const int flags = lane < NW ? s_left[lane].flags : 0;
+    const uint32_t closed = __ballot_sync(kFull, !(flags & kThrough)) & ~((1u << w0) | ((1u << w0) - 1u));
+    const bool through = chain > 0 || (first.flags & kThrough);
+    const int stop = through ? __ffs(closed) - 1 : w0;
+    const bool open = through && stop >= NW;
+    const int w1 = min(stop, NW - 1);
+    const uint32_t away = __ballot_sync(kFull, flags & kAway);
+    for (int i = threadIdx.x & 127; i < min(all - row0, P::kRows) * (D / 4); i += 128) {
       const int r = i / (D / 4), d = 4 * (i % (D / 4));
       float top = -INFINITY, sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int w = w0; w <= w1; ++w) {
-        const bool away = w >= chain && (s_left[w].flags & kAway);
-        const float* from =
-            away ? heads_of + w * P::kSums : reinterpret_cast<const float*>(smem + w * P::kWarpRing);
+      auto add = [&](const float* from) {
         add_sums(top, sum, v, from[P::kRows * P::kRow + r], from[P::kRows * P::kRow + P::kRows + r],
                  *reinterpret_cast<const float4*>(from + r * P::kRow + d));
+      };
+#pragma unroll 4
+      for (int w = w0; w <= w1; ++w) {
+        if (w >= chain && (away >> w & 1u))
+          add(heads_of + w * P::kSums);
+        else
+          add(reinterpret_cast<const float*>(smem + w * P::kWarpRing));
       }
       if (chain > 0 && !open) {
         finish(piece.b, kv_head, row0 + r, d, top, sum, v);
