@@ -189,6 +189,13 @@ __device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[1]) {
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
 }
 
+// ---------------------------------------------------------------- 32-byte stores
+__device__ __forceinline__ void st_32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // ---------------------------------------------------------------- predicated loads
 // v = (mask & bit) ? *p : 0, streaming (evict-first) global load
 __device__ __forceinline__ uint32_t ld_cs_if(const uint32_t* p, uint32_t mask, uint32_t bit) {
