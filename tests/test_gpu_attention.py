@@ -206,6 +206,25 @@ def test_cached_attention_long(lens, dim, group, heads, kv, new):
     check_cached(rand((len(lens), new, heads, dim), "bf16", 6, 0.3), case, group, "bf16")
 
 
+@pytest.mark.parametrize("dtype,limit", [("bf16", 3e-3), ("f16", 1e-3)])
+def test_cached_attention_long_and_flat(dtype, limit):
+    """Nearly equal weights over 131071 tokens: out is 1/900 of the codes' sum and the
+    zeros' that make it up, so what rounding costs those sums shows. In the 2-norm, relative to out:
+    out's own rounding 1.7e-3 (bf16) or 2.1e-4, the weights' 11 bits 7e-4 (2.5e-4 where the middle code is
+    given back), fp32 sums 900 x 2^-24 x the square root of the 64 steps of a run: 4.5e-4."""
+    n, page = 131071, 64
+    cache = G.grinqh_kv4_cache(2048, 1, 128, page, 128)
+    k, v = rand((n, 1, 128), dtype, 1), rand((n, 1, 128), dtype, 2, 0.0)
+    G.grinqh_kv4_append(k, v, cache, torch.arange(n).cuda(), 128)
+    q = rand((1, 4, 128), dtype, 3) * 0.05
+    out, lse = G.grinqh_kv4_attention(q, cache, torch.arange(2048, dtype=torch.int32).cuda()[None],
+                                      torch.tensor([n], dtype=torch.int32).cuda(), 128)
+    kr, vr = (x[:n, None] for x in A.read_tokens(cache.cpu().numpy().reshape(-1, cache.shape[-1]), 128, 128, dtype))
+    ref, ref_lse, _, _ = A.attention(q.double().cpu().numpy(), kr, vr, 128**-0.5)
+    assert np.linalg.norm(out.double().cpu().numpy() - ref) <= limit * np.linalg.norm(ref)
+    assert np.abs(lse.double().cpu().numpy() - ref_lse).max() <= 2.0**-20 * (1 + np.abs(ref_lse).max())
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_cached_attention_large_scores(dtype):
     """Scores of hundreds that rise along the sequence, and values of very different size."""

@@ -643,13 +643,10 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) l[n][c] += add[n][c];
+          // weights x scale as operand B of the output's product
+          uint32_t pf[2][NT][NG][2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t va[W], vb[W];
-            load_words(rec + i * L::kRecord + v_at, va);
-            load_words(rec + i * L::kRecord + 4 * D + v_at, vb);
-            // weights x scale as operand B of the output's product
-            uint32_t pf[NT][NG][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const float* w = p[i][n];
@@ -676,24 +673,38 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
                   z[n][0][k] = fmaf((u[0] - ra.x) + (u[2] - rb.x), 7.5f * back, z[n][0][k]);
                   z[n][1][k] = fmaf((u[1] - ra.y) + (u[3] - rb.y), 7.5f * back, z[n][1][k]);
                 }
-                pf[n][k][0] = transpose_8x8(ha);
-                pf[n][k][1] = transpose_8x8(hb);
+                pf[i][n][k][0] = transpose_8x8(ha);
+                pf[i][n][k][1] = transpose_8x8(hb);
               }
             }
-            // Rows g are fed the whole byte 16 hi + lo, rows g + 8 its 16 hi: their difference
-            // in the end is lo's sum, exact but for fp32's rounding, and an AND fewer per word.
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const uint32_t u = k == 0 ? va[w] & 0x00ff00ffu : __byte_perm(va[w], 0u, 0x4341u);
-                const uint32_t y = k == 0 ? vb[w] & 0x00ff00ffu : __byte_perm(vb[w], 0u, 0x4341u);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                  mma_m16n8k16(o[2 * w + k][n], u, u & 0x00f000f0u, y, y & 0x00f000f0u, pf[n][w / L::kGroupWords][0],
-                               pf[n][w / L::kGroupWords][1]);
-              }
           }
+          // The products of a step start from zero and are added to the sums here: the
+          // instruction cuts its sums off instead of rounding them, and over a long sequence,
+          // where the codes' sum and the zeros' all but cancel, that bias showed (1.6 % of
+          // the output at 131072 tokens when the sums stayed in it and lo was the difference
+          // of whole bytes and hi).
+          uint32_t va[2][W], vb[2][W];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            load_words(rec + i * L::kRecord + v_at, va[i]);
+            load_words(rec + i * L::kRecord + 4 * D + v_at, vb[i]);
+          }
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float acc[4];
+                const uint32_t u = va[0][w] >> (8 * k), y = vb[0][w] >> (8 * k);
+                mma_m16n8k16_zero(acc, u & 0x000f000fu, u & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u,
+                                  pf[0][n][w / L::kGroupWords][0], pf[0][n][w / L::kGroupWords][1]);
+                const uint32_t u1 = va[1][w] >> (8 * k), y1 = vb[1][w] >> (8 * k);
+                mma_m16n8k16(acc, u1 & 0x000f000fu, u1 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u,
+                             pf[1][n][w / L::kGroupWords][0], pf[1][n][w / L::kGroupWords][1]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[2 * w + k][n][c] += acc[c];
+              }
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[warp][get]);
           if (++get == ST) {
@@ -727,9 +738,9 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
               const int gi = w / L::kGroupWords, j = w % L::kGroupWords;
               const int d = gi * GS + g * (GS / 8) + 4 * j;
               const float f = back * 16777216.0f;
-              const float4 v = make_float4(fmaf(o[2 * w][n][c] - o[2 * w][n][2 + c], f, z[n][c][gi]),
+              const float4 v = make_float4(fmaf(o[2 * w][n][c], f, z[n][c][gi]),
                                            fmaf(o[2 * w][n][2 + c], f * 0.0625f, z[n][c][gi]),
-                                           fmaf(o[2 * w + 1][n][c] - o[2 * w + 1][n][2 + c], f, z[n][c][gi]),
+                                           fmaf(o[2 * w + 1][n][c], f, z[n][c][gi]),
                                            fmaf(o[2 * w + 1][n][2 + c], f * 0.0625f, z[n][c][gi]));
               if (began || goes) {
                 *reinterpret_cast<float4*>(sums + r * P::kRow + d) = v;
