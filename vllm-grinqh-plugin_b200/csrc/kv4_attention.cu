@@ -26,6 +26,11 @@
 // run is finished by its warp; the sums of one that several warps share are joined in
 // shared memory when the CTA's warps are done, and where it is shared by several CTAs,
 // each writes its sums to the workspace and the last one to arrive joins them in order.
+//
+// Measured (bf16, D = 128, group 128, 32 / 8 heads): 5 sequences of 50001 to 131072 tokens,
+// 111 us, 67% of the copy bandwidth (the loop runs at 90%; the rest is the ends, and the SMs
+// whose loads take longer); 64 of 512 to 768, group 64, 26 us, 28%; one of 301, 8 us, one
+// after another: looking up pages, a record, joining.
 #include "kv4.cuh"
 #include "kv4_attention.cuh"
 #include "launch.cuh"
@@ -82,6 +87,7 @@ struct Plan {
 };
 
 // What a sequence and head costs beside its records, in records: q, finishing or joining.
+// 33 sequences of up to 9000 tokens, 8 kv heads: 55.2 us with 4, 52.5 with 8, 53.9 with 16.
 constexpr int kCost = 8;
 
 __device__ __forceinline__ int tiles_of(const Kv4AttnArgs& a, int b) {
@@ -220,13 +226,15 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
     tiles = __reduce_add_sync(kFull, tiles) * heads;
     most = __reduce_max_sync(kFull, most);
     count = __reduce_add_sync(kFull, count) * heads;
-    // Even runs. Where a CTA for each sequence and head is hardly longer than that for
-    // the longest, it is taken: no sums pass between CTAs, which costs a few microseconds.
+    // Even runs. Where a CTA for each sequence and head makes the runs of the longest at
+    // most 2 records longer, that is taken: no sums pass between CTAs. Measured with 8 kv
+    // heads, D = 128: 18 sequences of 300 tokens, 16.0 us with even runs and 12.3 so, 18 of
+    // 4000, 32.8 and 28.7; 5 of 500 to 1500, 6 records longer, 16.2 and 18.4.
     const int workers = (int)gridDim.x * NW;
     int total = tiles + count * kCost;
     int per = max((total + workers - 1) / workers, 2), same = 0;
     const int alone = (most + NW - 1) / NW;
-    if (count <= (int)gridDim.x && alone <= per + 6) {
+    if (count <= (int)gridDim.x && alone <= per + 2) {
       per = max(alone, 1);
       same = per * NW;
       total = count * same;
@@ -930,7 +938,7 @@ extern "C" int grinqh_kv4_attention(const void* q, int dtype, int64_t num_seqs, 
                  "block_tables out of range");
   GRINQH_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "softmax_scale must be positive and finite");
   GRINQH_REQUIRE(2.0 * (double)num_seqs * num_kv_heads * ((double)table_width * (page_size / kTile) + kCost) < 2147000000.0,
-                 "num_seqs x num_kv_heads x (table_width x page_size / 16 + 6) must be below 1073000000");
+                 "num_seqs x num_kv_heads x (table_width x page_size / 16 + 8) must be below 1073000000");
   if (num_seqs == 0) return GRINQH_OK;
   GRINQH_REQUIRE(q && seq_lens && out && lse && (block_tables || table_width == 0), "null pointer");
   GRINQH_REQUIRE(aligned(q, 16) && q_seq_stride % 8 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0 &&

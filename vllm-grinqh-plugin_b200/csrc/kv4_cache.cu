@@ -7,6 +7,11 @@
 // so its rounding costs at most 15 * 2^-9 of a step at the group's largest value. The
 // quotient is a product with 1 / scale: a code can differ from the quotient's only where
 // x lies midway between two codes, to fp32 precision.
+//
+// Bound by HBM: 4 D bytes of K and V in the model's type and D + 8 NG of the cache, per
+// token and kv head. Measured with 8 kv heads: append of 16383 tokens, D = 128, group 128,
+// 49 us, 53% of the copy bandwidth; gather of 70001, D = 64, group 32, 41 us, 71%. 64
+// tokens, 13 us, and 1500 read back, 8 us, are the call on the host.
 #include "kv4.cuh"
 
 #include <algorithm>

@@ -174,21 +174,6 @@ __device__ __forceinline__ void prefetch_l2(const void* p) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
-// ---------------------------------------------------------------- shared loads
-// By 32-bit shared address (aligned to the size), ordered with the waits around them.
-__device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[4]) {
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-               : "r"(at)
-               : "memory");
-}
-__device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[2]) {
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void lds(uint32_t at, uint32_t (&w)[1]) {
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
-}
-
 // ---------------------------------------------------------------- 32-byte stores
 __device__ __forceinline__ void st_32(void* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
