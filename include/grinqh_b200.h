@@ -331,8 +331,9 @@ int grinqh_kv4_attention(const void *q, int dtype, int64_t num_seqs, int new_tok
  * contiguous; pointers and strides 16-byte aligned, out 32-byte; at most 128 query heads per
  * kv head.
  * workspace: as many bytes as grinqh_prompt_attention_workspace_size says (0 where no keys
- * are split), 256-byte aligned; its first 16 KiB are left as they are. A key or value that is not finite may
- * reach earlier queries of its own sequence (0 * inf is NaN), never another sequence. */
+ * are split), 256-byte aligned; its first 16 KiB are left as they are. A key or value that
+ * is not finite may reach earlier queries of its own sequence (0 * inf is NaN), never
+ * another sequence. */
 size_t grinqh_prompt_attention_workspace_size(int64_t total_q, int64_t total_k, int num_seqs, int num_heads,
                                               int num_kv_heads, int head_dim);
 int grinqh_prompt_attention(const void *q, const void *k, const void *v, int dtype, int64_t total_q, int64_t total_k,
