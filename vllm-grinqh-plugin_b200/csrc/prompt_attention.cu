@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
               __stcg(reinterpret_cast<uint4*>(sums) + (h + d) / 4 * kRows + r,
                      make_uint4(o[d], o[d + 1], o[d + 2], o[d + 3]));
           }
-          } else {
+        } else {
           uint32_t w0[8], w1[8];  // what this lane stores of the two rows
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
