@@ -32,8 +32,8 @@
 // cut into the same number of parts, items of their own; each writes its sums to the
 // workspace and a second kernel joins them in order.
 //
-// Measured (bf16, D = 128): a prompt of 16384 tokens, 8 / 2 heads, 480 us, 1.15 PFLOP/s or
-// 68% of a library matrix product's rate; 14 packed prompts of up to 2048 tokens, 32 / 8
+// Measured (bf16, D = 128): a prompt of 16384 tokens, 8 / 2 heads, 475 us, 1.16 PFLOP/s or
+// 69% of a library matrix product's rate; 14 packed prompts of up to 2048 tokens, 32 / 8
 // heads, 110 us, with the tensor pipe active in 46% of the cycles.
 //
 // Keys past the sequence's end belong to another sequence and may hold anything: their
@@ -78,6 +78,11 @@ struct Shape {
   static constexpr uint32_t kBytes = kAtoms * kAtom;
   static constexpr int kStages = D == 128 ? 5 : 10;      // K / V blocks in the ring
   static constexpr uint32_t kSmem = 2 * kQBytes + kStages * kBytes + 1024 /*align*/ + 512 /*barriers*/;
+  // Steps of 16 keys whose weights are handed over first, while the others are made. At
+  // head_dim 64 the exponentials bound the kernel and the wait for them is worth a second
+  // hand-over: chunks of prompts 69.4 -> 68.0 us with 64 keys first; at 128 the products do, and it
+  // costs: a prompt of 16384 tokens 487 -> 495.
+  static constexpr int kFirst = D == 64 ? kKeys / 32 : kKeys / 16;
   // TMEM columns: S, then P and O of both tiles
   static constexpr uint32_t kS = 0, kP = kKeys, kO = 2 * kKeys, kPNext = kKeys / 2, kONext = D;
   static_assert(kO + 2 * D <= kTmemCols && kSmem <= 227 * 1024, "budgets");
@@ -219,7 +224,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   uint64_t* s_full = q_empty + 1;   // [2] S of a tile is in TMEM
   uint64_t* s_empty = s_full + 2;   // ... is in registers
   uint64_t* p_full = s_empty + 1;   // [2] P of a tile is in TMEM
-  uint64_t* o_full = p_full + 2;    // [2] ... has been multiplied: O holds the block, P may be written
+  uint64_t* p_half = p_full + 2;    // [2] ... of the first kFirst steps
+  uint64_t* o_full = p_half + 2;    // [2] ... has been multiplied: O holds the block, P may be written
   uint64_t* o_empty = o_full + 2;   // [2] O of an item is read
   uint64_t* i_full = o_empty + 2;   // [2] an item is known
   uint64_t* i_empty = i_full + 2;   // [2] ... is not needed any more
@@ -242,6 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
     for (int t = 0; t < 2; ++t) {
       mbar_init(&s_full[t], 1);
       mbar_init(&p_full[t], 128);
+      mbar_init(&p_half[t], 128);
       mbar_init(&o_full[t], 1);
       mbar_init(&o_empty[t], 128);
       mbar_init(&i_full[t], 1);
@@ -367,23 +374,38 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         __syncwarp();
       };
       auto outputs = [&](int t, int at, int steps, bool more) {  // O_t += P_t V, steps of 16 keys
-        mbar_wait_nocall(&p_full[t], np[t] & 1);
-        ++np[t];
-        tc_fence_after();
         const uint64_t vd = v_desc + at * (S::kBytes >> 4);
         const uint32_t o = tm + S::kO + t * S::kONext, p = tm + S::kP + t * S::kPNext;
+        constexpr int kSteps = kKeys / 16, kFirst = S::kFirst;
+        mbar_wait_nocall(kFirst < kSteps ? &p_half[t] : &p_full[t], np[t] & 1);
+        tc_fence_after();
         if (elect_one()) {
-          if (steps == kKeys / 16) {
+          if (steps >= kFirst) {
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
+            for (int kk = 0; kk < kFirst; ++kk)
               mma_f16_ts(o, p + kk * 8, vd + kk * 128, id_o, more || kk > 0 ? 1u : 0u);
           } else {
             for (int kk = 0; kk < steps; ++kk)
               mma_f16_ts(o, p + kk * 8, vd + kk * 128, id_o, more || kk > 0 ? 1u : 0u);
           }
-          mma_commit(&o_full[t]);
+          if constexpr (kFirst == kSteps) mma_commit(&o_full[t]);
         }
         __syncwarp();
+        if constexpr (kFirst < kSteps) {
+          mbar_wait_nocall(&p_full[t], np[t] & 1);
+          tc_fence_after();
+          if (elect_one()) {
+            if (steps == kSteps) {
+#pragma unroll
+              for (int kk = kFirst; kk < kSteps; ++kk) mma_f16_ts(o, p + kk * 8, vd + kk * 128, id_o, 1u);
+            } else {
+              for (int kk = kFirst; kk < steps; ++kk) mma_f16_ts(o, p + kk * 8, vd + kk * 128, id_o, 1u);
+            }
+            mma_commit(&o_full[t]);
+          }
+          __syncwarp();
+        }
+        ++np[t];
       };
       int stage = 0, round = 0, used = 0;  // ring stage of the next block and its parity; items so far
       auto next = [&] {
@@ -494,9 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         const bool rescale = __any_sync(0xffffffffu, up);
         if (rescale) l0.x *= f, l0.y *= f, l1.x *= f, l1.y *= f;
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
-        uint32_t pk[kChunks][kCols / 2];
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
+        auto weights = [&](int c, uint32_t (&pk)[kCols / 2]) {
 #pragma unroll
           for (int i = 0; i < kCols / 2; ++i) {
             const float2 x = __ffma2_rn(
@@ -506,9 +526,12 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
               l1 = __fadd2_rn(l1, p);
             else
               l0 = __fadd2_rn(l0, p);
-            pk[c][i] = pack2<T>(p.x, p.y);
+            pk[i] = pack2<T>(p.x, p.y);
           }
-        }
+        };
+        uint32_t pk[kChunks][kCols / 2];
+#pragma unroll
+        for (int c = 0; c < S::kFirst; ++c) weights(c, pk[c]);
         // the weights stay in registers until the block before has been multiplied: P is
         // free then, and O whole
         if (ns > 0) mbar_wait_nocall(&o_full[t], (ns - 1) & 1);
@@ -525,7 +548,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
           }
         }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) tmem_st8(tp + kCols / 2 * c, pk[c]);
+        for (int c = 0; c < S::kFirst; ++c) tmem_st8(tp + kCols / 2 * c, pk[c]);
+        if constexpr (S::kFirst < kChunks) {  // their product may begin while the others are made
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&p_half[t]);
+#pragma unroll
+          for (int c = S::kFirst; c < kChunks; ++c) weights(c, pk[c]);
+#pragma unroll
+          for (int c = S::kFirst; c < kChunks; ++c) tmem_st8(tp + kCols / 2 * c, pk[c]);
+        }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_full[t]);
