@@ -199,7 +199,9 @@ __device__ __forceinline__ uint4 values8(uint32_t codes, uint32_t params) {
 
 // One lane per 8 channels of a token and head (blockIdx.y), the lanes of tokens 2 p and
 // 2 p + 1 side by side: where they are a pair in the cache too, both read the same words of
-// V. A thread takes kUnits pairs of tokens, for more loads in flight behind the slots'.
+// V. A thread takes kUnits pairs of tokens, for more loads in flight behind the slots': 70001
+// tokens, D = 64, 41.3 us with one, 40.8 with two, 40.9 with four. Nor do smaller blocks (40.7)
+// or stores that stay in L2 (40.2) change much: three quarters of the bytes are writes.
 template <typename T, int D, int GS>
 __global__ void __launch_bounds__(kThreads) gather_kernel(CacheArgs a, T* __restrict__ k, T* __restrict__ v) {
   using L = Kv4<D, GS>;
