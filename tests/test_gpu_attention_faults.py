@@ -1,0 +1,126 @@
+"""What a reading of the attention operators and of what they share with the linears found
+wrong, each held by a test: workspaces of captured graphs.
+"""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+from grinqh import attention as G  # noqa: E402
+from grinqh.kernel import grinqh_gemm_or_gemv  # noqa: E402
+from grinqh.utils import pack_codes  # noqa: E402
+
+
+def rand(shape, seed, dtype=torch.bfloat16, spread=0.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g) * torch.exp(spread * torch.randn(shape[-1:], generator=g))
+    return x.to(dtype).cuda()
+
+
+def filled_cache(lens, kv, dim, group, page, seed, dtype=torch.bfloat16):
+    """A cache with the sequences' random K and V, its tables and lengths."""
+    need = [-(-n // page) for n in lens]
+    cache = G.grinqh_kv4_cache(sum(need) + 1, kv, dim, page, group)
+    order = np.random.default_rng(seed).permutation(sum(need) + 1)
+    tables, at = np.zeros((len(lens), max(need)), np.int32), 0
+    for b, n in enumerate(lens):
+        tables[b, :need[b]] = order[at:at + need[b]]
+        at += need[b]
+        t = np.arange(n)
+        slots = torch.from_numpy(tables[b, t // page].astype(np.int64) * page + t % page).cuda()
+        G.grinqh_kv4_append(rand((n, kv, dim), seed + 2 * b, dtype), rand((n, kv, dim), seed + 2 * b + 1, dtype),
+                            cache, slots, group)
+    return cache, torch.from_numpy(tables).cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+
+
+# ------------------------------------------------------------------ workspaces of captured graphs
+def small_and_large(kind):
+    """A call with a workspace, and one on a larger workspace."""
+    if kind == "cached":
+        cache, tables, lens = filled_cache([4000, 9, 1200], 2, 128, 64, 64, 1)
+        few, many = rand((3, 8, 128), 2), rand((3, 4, 8, 128), 3)  # 4 query rows a kv head, and 16
+        return (lambda: G.grinqh_kv4_attention(few, cache, tables, lens, 64),
+                lambda: G.grinqh_kv4_attention(many, cache, tables, lens, 64))
+    if kind == "prompt":  # keys in 4 parts, and in 2 parts of four times the items
+        cu = [torch.tensor([0, n], dtype=torch.int32).cuda() for n in (40, 160, 6000)]
+        k, v = rand((6000, 8, 128), 4), rand((6000, 8, 128), 5)
+        few, many = rand((40, 32, 128), 6), rand((160, 32, 128), 7)
+        return (lambda: G.grinqh_prompt_attention(few, k, v, cu[0], cu[2]),
+                lambda: G.grinqh_prompt_attention(many, k, v, cu[1], cu[2]))
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w = pack_codes(torch.randint(-128, 128, (4096, 4096), dtype=torch.int8, device="cuda", generator=g), 8)
+    s = torch.full((32, 4096), 0.01, dtype=torch.bfloat16, device="cuda")
+    few, many = rand((16, 4096), 8), rand((512, 4096), 9)
+    return (lambda: (grinqh_gemm_or_gemv(few, w, s, None, 8, 128, 1024, [0.0] * 4),),
+            lambda: (grinqh_gemm_or_gemv(many, w, s, None, 8, 128, 1024, [0.0] * 4),))
+
+
+def graph_of(call, stream):
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        kept = call()
+    return graph, kept
+
+
+@pytest.mark.parametrize("kind", ["cached", "prompt", "linear"])
+def test_graph_outlives_its_streams_workspace(kind):
+    """A graph captured on a stream that has a workspace is replayed after a call on that
+    stream has had it replaced by a larger one and its memory has been given to tensors."""
+    few, many = small_and_large(kind)
+    stream = torch.cuda.Stream(priority=-1)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        want = [x.clone() for x in few()]
+    graph, kept = graph_of(few, stream)
+    with torch.cuda.stream(stream):
+        many()
+        others = [torch.full((n,), 0xA5, dtype=torch.uint8, device="cuda") for n in (1 << 20, 8 << 20, 10 << 20) for _ in range(6)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for x in kept:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(kept, want))
+    assert all(bool((x == 0xA5).all()) for x in others)
+
+
+@pytest.mark.parametrize("kind", ["cached", "prompt", "linear"])
+def test_graph_replays_beside_calls_on_its_stream(kind):
+    """A replay on one stream and calls on the stream that it was captured on, at one time."""
+    few, _ = small_and_large(kind)
+    stream, other = torch.cuda.Stream(priority=-1), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        want = [x.clone() for x in few()]
+    graph, kept = graph_of(few, stream)
+    outs = []
+    for _ in range(30):
+        with torch.cuda.stream(other):
+            graph.replay()
+            outs.append([x.clone() for x in kept])
+        with torch.cuda.stream(stream):
+            outs.append(few())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for out in outs for x, y in zip(out, want))
+
+
+def test_graph_of_several_calls():
+    """Calls of different sizes in one capture, the larger ones behind the smaller."""
+    pairs = [small_and_large(kind) for kind in ("linear", "cached", "prompt")]
+    calls = [call for pair in pairs for call in pair]
+    want = [[x.clone() for x in call()] for call in calls]
+    graph, kept = graph_of(lambda: [call() for call in calls + calls], torch.cuda.Stream())
+    for _ in range(3):
+        for out in kept:
+            for x in out:
+                x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for out, ref in zip(kept, want + want):
+            assert all(torch.equal(x, y) for x, y in zip(out, ref))

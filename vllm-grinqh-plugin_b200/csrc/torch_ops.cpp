@@ -62,31 +62,50 @@ cudaStream_t cur_stream(const at::Tensor& t) {
   return at::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
 
-// A zeroed workspace per (device, stream), grown on demand and kept for the process.
-// The kernels leave their split-K tickets at zero, so a call that reuses it passes
+// A workspace whose tickets are zero, per (device, stream), grown on demand and kept for the
+// process. The kernels leave their split-K tickets at zero, so a call that reuses it passes
 // GRINQH_WORKSPACE_ZEROED and no clearing runs on the stream; calls on one stream are
-// ordered, and other streams get their own. A workspace is only created outside
-// stream capture (a capture records the zeroing instead of running it): a call
-// captured before any eager call on its stream allocates per call as before.
+// ordered, and other streams get their own.
+//
+// A capture gets a workspace of its own on each of its streams, from the graph's memory and
+// cleared by the graph: a replay may run on any stream, beside calls on the one that it was
+// captured on, and after the workspace of that one has been replaced by a larger one.
 at::Tensor stream_workspace(const at::Tensor& like, size_t bytes, cudaStream_t st, bool* zeroed) {
+  struct Captured {
+    unsigned long long id;
+    at::Tensor workspace;
+  };
+  constexpr size_t kTicketBytes = 16 << 10;  // where every call keeps its tickets
   static std::mutex mu;
   static std::map<std::pair<int, uintptr_t>, at::Tensor> cache;
-  std::lock_guard<std::mutex> lk(mu);
+  static std::map<std::pair<int, uintptr_t>, Captured> captured;
   const auto key = std::make_pair(static_cast<int>(like.device().index()), reinterpret_cast<uintptr_t>(st));
-  auto it = cache.find(key);
-  if (it != cache.end() && static_cast<size_t>(it->second.numel()) >= bytes) {
-    *zeroed = true;
-    return it->second;
-  }
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone) {
-    *zeroed = false;
-    return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
-  }
-  const size_t size = std::max<size_t>(bytes, size_t(1) << 20);
-  at::Tensor t = at::zeros({static_cast<int64_t>(size)}, like.options().dtype(at::kByte));
-  cache[key] = t;
+  unsigned long long id = 0;
+  // (the legacy stream has no answer while a blocking stream captures; it does not itself)
+  const bool known = cudaStreamGetCaptureInfo(st, &cap, &id) == cudaSuccess;
+  if (!known) cudaGetLastError();
+  const bool capturing = known && cap != cudaStreamCaptureStatusNone;
+  std::lock_guard<std::mutex> lk(mu);
   *zeroed = true;
+  const auto kept = captured.find(key);
+  if (kept != captured.end()) {
+    if (capturing && kept->second.id == id) {
+      if (static_cast<size_t>(kept->second.workspace.numel()) >= bytes) return kept->second.workspace;
+    } else {
+      captured.erase(kept);  // of a capture that has ended: the graph's own memory holds it
+    }
+  }
+  const auto it = cache.find(key);
+  if (!capturing && it != cache.end() && static_cast<size_t>(it->second.numel()) >= bytes) return it->second;
+  const size_t size = std::max<size_t>(bytes, size_t(1) << 20);
+  at::Tensor t = at::empty({static_cast<int64_t>(size)}, like.options().dtype(at::kByte));
+  const cudaError_t c = cudaMemsetAsync(t.data_ptr(), 0, kTicketBytes, st);
+  TORCH_CHECK(c == cudaSuccess, "GRINQH: cudaMemsetAsync: ", cudaGetErrorString(c));
+  if (capturing)
+    captured[key] = Captured{id, t};
+  else
+    cache[key] = t;
   return t;
 }
 
