@@ -1,5 +1,6 @@
 """What a reading of the attention operators and of what they share with the linears found
-wrong, each held by a test: workspaces of captured graphs.
+wrong, each held by a test: workspaces of captured graphs,
+caches without heads.
 """
 import numpy as np
 import pytest
@@ -124,3 +125,19 @@ def test_graph_of_several_calls():
         torch.cuda.synchronize()
         for out, ref in zip(kept, want + want):
             assert all(torch.equal(x, y) for x, y in zip(out, ref))
+
+
+# ------------------------------------------------------------------ refusals
+def test_cache_without_heads_is_refused():
+    cache = G.grinqh_kv4_cache(4, 0, 128, 16, 128)
+    none = torch.zeros(3, 0, 128, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(1, 8, 128, dtype=torch.bfloat16, device="cuda")
+    tables, lens = torch.zeros(1, 4, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError):
+        G.grinqh_kv4_attention(q, cache, tables, lens)
+    with pytest.raises(RuntimeError):
+        G.grinqh_kv4_attention(q[:, :0], cache, tables, lens)
+    with pytest.raises(RuntimeError):
+        G.grinqh_kv4_append(none, none, cache, torch.arange(3).cuda())
+    with pytest.raises(RuntimeError):
+        G.grinqh_prompt_attention(q, none[:1], none[:1], lens, lens)

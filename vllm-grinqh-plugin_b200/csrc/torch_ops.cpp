@@ -548,6 +548,7 @@ std::tuple<at::Tensor, at::Tensor> kv4_attention(const at::Tensor& q, const at::
   TORCH_CHECK(block_tables.size(0) == seqs && seq_lens.size(0) == seqs, "GRINQH: block_tables and seq_lens must have ",
               seqs, " rows, got ", block_tables.size(0), " and ", seq_lens.size(0));
   const c10::cuda::CUDAGuard guard(q.device());
+  TORCH_CHECK(c.kv_heads > 0, "GRINQH: the cache has no kv heads");
   const at::Tensor qc = rows16(q), lens = seq_lens.contiguous();
   const at::Tensor tables = block_tables.stride(1) == 1 ? block_tables : block_tables.contiguous();
   at::Tensor out = at::empty(q.sizes(), q.options());
