@@ -328,8 +328,8 @@ int grinqh_kv4_attention(const void *q, int dtype, int64_t num_seqs, int new_tok
  * are the last of its m tokens: query j sees keys 0 .. m - n + j. Formulas, out and lse as
  * for grinqh_kv4_attention; out [total_q, num_heads, D] and lse [total_q, num_heads] are
  * contiguous, and rows that no sequence holds are not written. Strides in elements, D
- * contiguous; pointers and strides 16-byte aligned, out 32-byte; at most 128 query heads per
- * kv head.
+ * contiguous; pointers and strides 16-byte aligned, out 32-byte; strides positive; at most
+ * 128 query heads per kv head.
  * workspace: as many bytes as grinqh_prompt_attention_workspace_size says (0 where no keys
  * are split), 256-byte aligned; its first 16 KiB are left as they are. A key or value that
  * is not finite may reach earlier queries of its own sequence (0 * inf is NaN), never

@@ -1,6 +1,6 @@
 """What a reading of the attention operators and of what they share with the linears found
 wrong, each held by a test: workspaces of captured graphs,
-caches without heads.
+caches without heads, expanded inputs.
 """
 import numpy as np
 import pytest
@@ -141,3 +141,36 @@ def test_cache_without_heads_is_refused():
         G.grinqh_kv4_append(none, none, cache, torch.arange(3).cuda())
     with pytest.raises(RuntimeError):
         G.grinqh_prompt_attention(q, none[:1], none[:1], lens, lens)
+
+
+# ------------------------------------------------------------------ strides
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_of_expanded_and_transposed_inputs(dim):
+    """K and V of one head expanded over the kv heads, of one token over all; and q, k, v
+    held head by head."""
+    cu = torch.tensor([0, 70, 203], dtype=torch.int32).cuda()
+    q, k, v = rand((203, 8, dim), 1), rand((203, 4, dim), 2), rand((203, 4, dim), 3)
+
+    def same(q, k, v):
+        got = G.grinqh_prompt_attention(q, k, v, cu, cu)
+        want = G.grinqh_prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu, cu)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+    same(q, k[:, :1].expand(-1, 4, -1), v[:, :1].expand(-1, 4, -1))
+    same(q[:1].expand(203, -1, -1), k[:1].expand(203, -1, -1), v)
+    same(q[:, :1].expand(-1, 8, -1), k, v)
+    same(*(x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)))
+
+
+def test_cache_of_expanded_inputs():
+    one, tokens = rand((40, 1, 128), 1), rand((1, 4, 128), 2)
+    slots = torch.arange(40).cuda()
+    caches = [G.grinqh_kv4_cache(3, 4, 128, 16, 64) for _ in range(2)]
+    G.grinqh_kv4_append(one.expand(-1, 4, -1), tokens.expand(40, -1, -1), caches[0], slots, 64)
+    G.grinqh_kv4_append(one.expand(-1, 4, -1).contiguous(), tokens.expand(40, -1, -1).contiguous(), caches[1], slots, 64)
+    assert torch.equal(*caches)
+    tables, lens = torch.arange(3, dtype=torch.int32).cuda()[None].expand(2, -1), torch.tensor([40, 17]).int().cuda()
+    q = rand((2, 1, 128), 3).expand(-1, 8, -1)
+    got = G.grinqh_kv4_attention(q, caches[0], tables, lens, 64)
+    want = G.grinqh_kv4_attention(q.contiguous(), caches[0], tables.contiguous(), lens, 64)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -33,6 +33,8 @@ inline int tmap_heads(CUtensorMap* map, bool bf16, const void* base, int64_t tok
   // a stride that no index is multiplied with may hold anything
   if (heads == 1) head_stride = dim;
   if (tokens == 1) token_stride = heads * dim;
+  GRINQH_REQUIRE(head_stride > 0 && token_stride > 0, "the strides of %s must be positive (got %lld, %lld)", what,
+                 (long long)token_stride, (long long)head_stride);
   const cuuint64_t gdim[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
   const cuuint64_t gstride[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
   const cuuint32_t box[3] = {64, box_heads, box_tokens}, step[3] = {1, 1, 1};

@@ -465,6 +465,13 @@ at::Tensor rows16(const at::Tensor& t) {
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
+// The same for a tensor map, which has no strides of 0: what was expanded is copied.
+at::Tensor mapped16(const at::Tensor& t) {
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.stride(i) == 0 && t.size(i) > 1) return t.clone(at::MemoryFormat::Contiguous);
+  return rows16(t);
+}
+
 struct CacheShape {
   int64_t pages, kv_heads, dim;
   int page_size;
@@ -541,6 +548,7 @@ std::tuple<at::Tensor, at::Tensor> kv4_attention(const at::Tensor& q, const at::
               "head_dim], got ", q.sizes());
   const int64_t seqs = q.size(0), fresh = q.dim() == 4 ? q.size(1) : 1, heads = q.size(-2);
   TORCH_CHECK(q.size(-1) == c.dim, "GRINQH: q has head_dim ", q.size(-1), " but the cache ", c.dim);
+  TORCH_CHECK(c.kv_heads > 0, "GRINQH: the cache has no kv heads");
   TORCH_CHECK(heads > 0 && fresh > 0 && heads % c.kv_heads == 0, "GRINQH: ", heads,
               " query heads are not a multiple of ", c.kv_heads, " kv heads (or there is no token)");
   check_index(block_tables, "block_tables", at::kInt, 2, q);
@@ -548,7 +556,6 @@ std::tuple<at::Tensor, at::Tensor> kv4_attention(const at::Tensor& q, const at::
   TORCH_CHECK(block_tables.size(0) == seqs && seq_lens.size(0) == seqs, "GRINQH: block_tables and seq_lens must have ",
               seqs, " rows, got ", block_tables.size(0), " and ", seq_lens.size(0));
   const c10::cuda::CUDAGuard guard(q.device());
-  TORCH_CHECK(c.kv_heads > 0, "GRINQH: the cache has no kv heads");
   const at::Tensor qc = rows16(q), lens = seq_lens.contiguous();
   const at::Tensor tables = block_tables.stride(1) == 1 ? block_tables : block_tables.contiguous();
   at::Tensor out = at::empty(q.sizes(), q.options());
@@ -591,7 +598,7 @@ std::tuple<at::Tensor, at::Tensor> prompt_attention(const at::Tensor& q, const a
               "GRINQH: cu_seqlens_q and cu_seqlens_k must both have one entry more than there are sequences, got ",
               cu_seqlens_q.size(0), " and ", cu_seqlens_k.size(0));
   const c10::cuda::CUDAGuard guard(q.device());
-  const at::Tensor qc = rows16(q), kc = rows16(k), vc = rows16(v);
+  const at::Tensor qc = mapped16(q), kc = mapped16(k), vc = mapped16(v);
   const at::Tensor cq = cu_seqlens_q.contiguous(), ck = cu_seqlens_k.contiguous();
   at::Tensor out = at::empty(q.sizes(), q.options());
   at::Tensor lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
