@@ -1,6 +1,6 @@
 """What a reading of the attention operators and of what they share with the linears found
 wrong, each held by a test: workspaces of captured graphs,
-caches without heads, expanded inputs.
+caches without heads, expanded inputs, joins of many sequences in a CTA.
 """
 import numpy as np
 import pytest
@@ -174,3 +174,22 @@ def test_cache_of_expanded_inputs():
     got = G.grinqh_kv4_attention(q, caches[0], tables, lens, 64)
     want = G.grinqh_kv4_attention(q.contiguous(), caches[0], tables.contiguous(), lens, 64)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ------------------------------------------------------------------ joins
+@pytest.mark.parametrize("dim,group", [(128, 32), (128, 64), (64, 32)])
+def test_cached_attention_of_many_short_sequences(dim, group):
+    """Every CTA holds many sequences and heads that several of its warps share: each is what
+    the sequence gives alone, up to the order of fp32 sums."""
+    lens = [37 + 11 * (i % 23) for i in range(400)]
+    cache, tables, start = filled_cache(lens, 2, dim, group, 32, 5)
+    q = rand((400, 8, dim), 6)
+    out, lse = G.grinqh_kv4_attention(q, cache, tables, start, group)
+    for _ in range(3):
+        again = G.grinqh_kv4_attention(q, cache, tables, start, group)
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    for b in list(range(0, 400, 37)) + [399]:
+        one = G.grinqh_kv4_attention(q[b:b + 1], cache, tables[b:b + 1], start[b:b + 1], group)
+        # weights in 11 bits and one rounding to bf16 on each side; codes x scale reach 3 x the values, 5 sigma
+        assert (out[b:b + 1] - one[0]).abs().max() <= 2 * (2.0**-11 * 15 + 2.0**-8 * one[0].abs().max())
+        assert (lse[b:b + 1] - one[1]).abs().max() <= 1e-5 * (1 + one[1].abs().max())

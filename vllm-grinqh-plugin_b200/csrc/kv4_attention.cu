@@ -780,10 +780,10 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
   // leaves open; a chain takes the heads of the warps behind it while they go through.
   // A thread takes 4 channels of a row of a chain.
   const int all = a.fresh * a.group;
-  // four warps a chain, as many chains at a time as there are
+  // four warps a chain, as many chains at a time as there are such; the rest of 15 have none
   constexpr int kGroups = (NW + 1) / 4;
   const bool is = lane <= NW && (s_left[max(lane - 1, 0)].flags & (lane == 0 ? kHead : kTail));
-  uint32_t chains = __ballot_sync(kFull, is);
+  uint32_t chains = __ballot_sync(kFull, is && warp < 4 * kGroups);
   for (int k = warp / 4; k > 0; --k) chains &= chains - 1u;
 #pragma unroll 1
   while (chains != 0u) {
