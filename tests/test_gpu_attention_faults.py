@@ -1,6 +1,7 @@
 """What a reading of the attention operators and of what they share with the linears found
 wrong, each held by a test: workspaces of captured graphs,
-caches without heads, expanded inputs, joins of many sequences in a CTA.
+caches without heads, expanded inputs, joins of many sequences in a CTA, a block
+that is full.
 """
 import numpy as np
 import pytest
@@ -193,3 +194,26 @@ def test_cached_attention_of_many_short_sequences(dim, group):
         # weights in 11 bits and one rounding to bf16 on each side; codes x scale reach 3 x the values, 5 sigma
         assert (out[b:b + 1] - one[0]).abs().max() <= 2 * (2.0**-11 * 15 + 2.0**-8 * one[0].abs().max())
         assert (lse[b:b + 1] - one[1]).abs().max() <= 1e-5 * (1 + one[1].abs().max())
+
+
+# ------------------------------------------------------------------ the block
+def test_block_refuses_tokens_behind_its_pages():
+    """One page of 16 tokens a sequence: what does not fit is refused on the host, and leaves
+    the block as it was."""
+    from grinqh.attention_block import AttentionBlock
+    block = AttentionBlock(2, 10, hidden=512, heads=4, kv_heads=2, head_dim=64, page=16, group=32)
+    rows = lambda n: rand((n, 512), n)  # noqa: E731
+    for bad in (0, 3, 34):
+        with pytest.raises(ValueError):
+            block.prompt(rows(bad))
+    block.prompt(rows(30))
+    cache = block.cache.clone()
+    for call, n in ((block.prompt, 4), (block.token, 4), (block.token, 1)):
+        with pytest.raises(ValueError):
+            call(rows(n))
+    assert block.length == 15 and torch.equal(block.cache, cache)
+    block.token(rows(2))
+    for call in (block.token, block.prompt):
+        with pytest.raises(ValueError):
+            call(rows(2))
+    assert block.length == 16 and block.lens.tolist() == [16, 16]

@@ -66,6 +66,16 @@ class AttentionBlock:
         t = torch.arange(first, first + count, device="cuda")
         return (self.tables[:, t // self.page].long() * self.page + t % self.page).flatten()
 
+    def _count(self, x: torch.Tensor) -> int:
+        """New tokens of every sequence in x; their places must be on its pages (an index behind
+        them would be a device fault)."""
+        count, rest = divmod(x.shape[0], self.seqs)
+        if rest or not count:
+            raise ValueError(f"GRINQH: {x.shape[0]} rows are not a positive multiple of {self.seqs} sequences")
+        if self.length + count > self.tables.shape[1] * self.page:
+            raise ValueError(f"GRINQH: {self.length} + {count} tokens do not fit {self.tables.shape[1]} pages of {self.page}")
+        return count
+
     def _project(self, x: torch.Tensor, count: int):
         q, k, v = self.qkv(x).view(-1, self.heads + 2 * self.kv, self.dim).split([self.heads, self.kv, self.kv], 1)
         pos = torch.arange(self.length, self.length + count, device="cuda").repeat(self.seqs)
@@ -74,7 +84,7 @@ class AttentionBlock:
     def prompt(self, x: torch.Tensor) -> torch.Tensor:
         """x [seqs * count, hidden], the next tokens of every sequence, packed: causal over
         themselves and what the cache holds of their prefix."""
-        count = x.shape[0] // self.seqs
+        count = self._count(x)
         q, k, v = self._project(x, count)
         ends = torch.arange(self.seqs + 1, dtype=torch.int32, device="cuda")
         keys, values = k, v
@@ -89,6 +99,8 @@ class AttentionBlock:
 
     def token(self, x: torch.Tensor) -> torch.Tensor:
         """x [seqs, hidden]: one more token of every sequence, over the cache."""
+        if self._count(x) != 1:
+            raise ValueError(f"GRINQH: {x.shape[0]} rows, but a token of each of {self.seqs} sequences was expected")
         q, k, v = self._project(x, 1)
         self._append(k, v, 1)
         out, _ = grinqh_kv4_attention(q, self.cache, self.tables, self.lens, self.group)
