@@ -1,7 +1,7 @@
 """What a reading of the attention operators and of what they share with the linears found
 wrong, each held by a test: workspaces of captured graphs,
 caches without heads, expanded inputs, joins of many sequences in a CTA, a block
-that is full.
+that is full, waits that are lost.
 """
 import numpy as np
 import pytest
@@ -15,6 +15,13 @@ if not torch.cuda.is_available():
 from grinqh import attention as G  # noqa: E402
 from grinqh.kernel import grinqh_gemm_or_gemv  # noqa: E402
 from grinqh.utils import pack_codes  # noqa: E402
+
+
+@pytest.fixture(autouse=True)
+def no_wait_is_lost():
+    G.grinqh_check_waits()
+    yield
+    G.grinqh_check_waits()
 
 
 def rand(shape, seed, dtype=torch.bfloat16, spread=0.0):
@@ -217,3 +224,43 @@ def test_block_refuses_tokens_behind_its_pages():
         with pytest.raises(ValueError):
             call(rows(2))
     assert block.length == 16 and block.lens.tolist() == [16, 16]
+
+
+# ------------------------------------------------------------------ waits
+def lost_rows(call, want, monkeypatch):
+    """Runs `call` with waits that give up at their first look, `want` being what it returns
+    without: each row is right or NaN, the loss is reported once, and later calls are right."""
+    monkeypatch.setenv("GRINQH_ATTENTION_WAIT_US", "0")
+    outs = [call() for _ in range(3)]
+    torch.cuda.synchronize()
+    monkeypatch.delenv("GRINQH_ATTENTION_WAIT_US")
+    again = call()  # the flag of the lost calls is still up
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    with pytest.raises(RuntimeError, match="gave up"):
+        G.grinqh_check_waits()
+    G.grinqh_check_waits()
+    lost = 0
+    for out, lse in outs:
+        gone = lse.isnan()
+        assert torch.equal(gone, out.isnan().all(-1)) and torch.equal(gone, out.isnan().any(-1))
+        assert torch.equal(out[~gone], want[0][~gone]) and torch.equal(lse[~gone], want[1][~gone])
+        lost += int(gone.sum())
+    assert lost > 0
+
+
+@pytest.mark.parametrize("lens,dim,group,new", [([20000, 3, 9000], 128, 64, 1), ([700] * 40, 128, 32, 1), ([50, 0, 31], 64, 32, 4),
+                                                ([5000, 800], 128, 128, 4)])
+def test_cached_attention_waits_are_bounded(lens, dim, group, new, monkeypatch):
+    cache, tables, seq = filled_cache(lens, 2, dim, group, 64, 11)
+    q = rand((len(lens), new, 8, dim), 12)
+    call = lambda: G.grinqh_kv4_attention(q, cache, tables, seq, group)  # noqa: E731
+    lost_rows(call, call(), monkeypatch)
+
+
+def test_check_of_waits_is_not_captured():
+    x = torch.zeros(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError):
+            G.grinqh_check_waits()

@@ -27,6 +27,9 @@
 // shared memory when the CTA's warps are done, and where it is shared by several CTAs,
 // each writes its sums to the workspace and the last one to arrive joins them in order.
 //
+// Waits are bounded. A warp whose wait is lost leaves NaN sums, so that the rows which
+// needed the record become NaN, and every CTA still arrives where it is waited for.
+//
 // Measured (bf16, D = 128, group 128, 32 / 8 heads): 5 sequences of 50001 to 131072 tokens,
 // 111 us, 67% of the copy bandwidth (the loop runs at 90%; the rest is the ends, and the SMs
 // whose loads take longer); 64 of 512 to 768, group 64, 26 us, 28%; one of 301, 8 us, one
@@ -66,6 +69,7 @@ struct Kv4AttnArgs {
   int page_tiles;
   int max_len;
   float scale_log2;  // softmax scale * log2(e)
+  uint64_t wait_ns;  // the longest wait
 };
 
 template <int D, int GS, int NT>
@@ -197,6 +201,7 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
   __shared__ int s_plan[3];  // places of a run, the common stride (0: none), places in all
   __shared__ Left s_left[NW];
   __shared__ int s_last[2];
+  __shared__ int s_lost;  // a wait of this CTA was lost
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -209,6 +214,8 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
     fence_mbar_init();
     s_left[warp].flags = 0;
   }
+
+  if (threadIdx.x == 0) s_lost = 0;
 
   // the next kernel's set-up may overlap this one, as this one's did its predecessor
   allow_dependent_grid();
@@ -391,16 +398,23 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
         idle = 0;
       } else {
         __nanosleep(20);
-        if ((++idle & 4095u) == 1u) {  // bounded, like every wait
+        if ((++idle & 63u) == 0u) {  // bounded, like every wait
           const uint64_t now = globaltimer_ns();
-          if (idle == 1u) since = now;
-          const bool late = now - since > kWaitNs || *reinterpret_cast<volatile unsigned*>(&g_wait_timeouts) != 0u;
-          if (__any_sync(kFull, late)) {
-            if (lane == 0) atomicAdd(&g_wait_timeouts, 1u);
-            break;
+          if (idle == 64u) since = now;
+          bool lost = *reinterpret_cast<volatile int*>(&s_lost) != 0;
+          if (!lost && now - since >= a.wait_ns) {
+            lost = true;
+            if (atomicExch(&s_lost, 1) == 0) atomicAdd(&g_wait_timeouts, 1u);
           }
+          if (__any_sync(kFull, lost)) break;
         }
       }
+    }
+    // the copies still in flight: of each stage the last, a round back behind `put`
+    if (lane < NW) {
+#pragma unroll 1
+      for (int s = 0; s < ST; ++s)
+        if (!mbar_drain(&s_full[lane][s], s < put ? phase ^ 1u : phase)) s_lost = 1;
     }
   } else {
     // -------------------------------------------------------------- a run, piece by piece
@@ -412,6 +426,7 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
                    v_at = L::kV + t * D + (g ^ (2 * t)) * (4 * W);
     int get = 0;
     uint32_t phase = 0;
+    bool lost = false;  // a wait of this warp was: no record is used from there on
     while (x < end) {
       const int t0 = seg.at, t1 = min(seg.nt, seg.at + (end - x));  // this piece's records
       if (t0 < t1) {
@@ -513,7 +528,8 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
         const int clear = min(t1, see / kTile);  // records before this one are seen whole by all rows
 #pragma unroll 1
         for (int tile = t0; tile < t1; tile += 2) {
-          mbar_wait_nocall(&s_full[warp][get], phase);
+          lost = lost || !__all_sync(kFull, mbar_wait_or_lose(&s_full[warp][get], phase, a.wait_ns, &s_lost));
+          if (lost) break;
           const unsigned char* rec = ring + get * P::kStage;
           const uint32_t gone = s_gone[warp][get];
           const bool masked = tile + 2 > clear || gone != 0u;  // a row does not see a token, or there is none
@@ -737,6 +753,7 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
 #pragma unroll
               for (int i = 0; i < NG; ++i) z[n][c][i] += __shfl_xor_sync(kFull, z[n][c][i], k);
             }
+            if (lost) l[n][c] = __int_as_float(0x7fffffff);  // NaN: so is what the rows come to
             if ((began || goes) && g == 0) {
               sums[P::kRows * P::kRow + r] = m[n][c];
               sums[P::kRows * P::kRow + P::kRows + r] = l[n][c];
@@ -780,6 +797,7 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
   // leaves open; a chain takes the heads of the warps behind it while they go through.
   // A thread takes 4 channels of a row of a chain.
   const int all = a.fresh * a.group;
+  const bool lost = s_lost != 0;
   // four warps a chain, as many chains at a time as there are such; the rest of 15 have none
   constexpr int kGroups = (NW + 1) / 4;
   const bool is = lane <= NW && (s_left[max(lane - 1, 0)].flags & (lane == 0 ? kHead : kTail));
@@ -816,6 +834,8 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
         else
           add(reinterpret_cast<const float*>(smem + w * P::kWarpRing));
       }
+      // a copy may have come to a ring after the sums: none of this CTA's count
+      if (lost) sum = __int_as_float(0x7fffffff);
       if (chain > 0 && !open) {
         finish(piece.b, kv_head, row0 + r, d, top, sum, v);
       } else {
@@ -974,6 +994,7 @@ extern "C" int grinqh_kv4_attention(const void* q, int dtype, int64_t num_seqs, 
   a.page_tiles = page_size / kTile;
   a.max_len = (int)(table_width * page_size);
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.wait_ns = attention_wait_ns();
   if (!(flags & GRINQH_WORKSPACE_ZEROED)) {
     const cudaError_t e = cudaMemsetAsync(workspace, 0, (size_t)sms * sizeof(unsigned), stream);
     if (e != cudaSuccess) return set_error(GRINQH_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));

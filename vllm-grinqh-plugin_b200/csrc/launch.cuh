@@ -2,10 +2,13 @@
 // programmatic dependent launch.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
+#include <cstdlib>
 #include <utility>
 
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace grinqh {
 
@@ -20,6 +23,13 @@ inline int allow_smem(const void* kern, std::atomic<uint64_t>& done, size_t byte
   }
   if (e != cudaSuccess) return set_error(GRINQH_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
   return GRINQH_OK;
+}
+
+// How long a wait within an attention kernel lasts before it is lost: GRINQH_ATTENTION_WAIT_US
+// microseconds (read on every call), by default 2 s.
+inline uint64_t attention_wait_ns() {
+  const char* e = std::getenv("GRINQH_ATTENTION_WAIT_US");
+  return e ? (uint64_t)std::max(0ll, std::min(std::atoll(e), 2000000ll)) * 1000 : kWaitNs;
 }
 
 // SMs of the current device (148 without one).

@@ -106,6 +106,36 @@ static __device__ __noinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   }
 }
 
+// A wait that a CTA can lose: true when the phase completes; false after `limit` ns (with 0
+// one look is taken), or when another wait of the CTA has been lost (`lost`, in shared
+// memory, set and counted by the first). What it waited for may then not be used: the caller
+// makes its outputs NaN and waits for its own copies (mbar_drain). Inline as a whole, since
+// a kernel that splits its registers between warps (setmaxnreg) can call no function.
+__device__ __forceinline__ bool mbar_wait_or_lose(uint64_t* bar, uint32_t parity, uint64_t limit, int* lost) {
+  if (limit == 0 ? mbar_test(bar, parity) : mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+  while (*reinterpret_cast<volatile int*>(lost) == 0) {
+    if (globaltimer_ns() - t0 >= limit) {
+      if (atomicExch(lost, 1) == 0) atomicAdd(&g_wait_timeouts, 1u);
+      return false;
+    }
+    if (mbar_try_wait(bar, parity)) return true;
+  }
+  return false;
+}
+
+// Waits for copies or products that still write this CTA's memory, whatever was lost.
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+  while (globaltimer_ns() - t0 < 4 * kWaitNs)
+    if (mbar_try_wait(bar, parity)) return true;
+  atomicAdd(&g_wait_timeouts, 1u);
+  return false;
+}
+
 // mbar_wait inline as a whole: a kernel that splits its registers between warps
 // (setmaxnreg) can call no function.
 __device__ __forceinline__ bool mbar_wait_nocall(uint64_t* bar, uint32_t parity) {

@@ -5,18 +5,22 @@ The reference leaves attention to vLLM; these operators are for hosts that own t
 decoder layer and want the cache as small as GRINQH's weights. A cache is a uint8 tensor
 [pages, kv heads, page_size / 16, record] (``grinqh_kv4_cache``); its layout is in
 ``include/grinqh_b200.h``. Every function raises on CPU tensors, runs on the current
-stream without synchronising, and can be recorded into a CUDA graph.
+stream without synchronising, and can be recorded into a CUDA graph. Waits inside the
+kernels are bounded (2 s, or ``GRINQH_ATTENTION_WAIT_US``); rows of ``kv4_attention`` whose wait was lost
+come out as NaN, and ``grinqh_check_waits`` raises.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
 
 from . import kernel  # noqa: F401  (loads the op library)
+from ._ext import cabi
 
 __all__ = ["grinqh_kv4_cache", "grinqh_kv4_append", "grinqh_kv4_gather", "grinqh_kv4_attention",
-           "grinqh_prompt_attention"]
+           "grinqh_prompt_attention", "grinqh_check_waits"]
 
 
 def _record_bytes(head_dim: int, group_size: int) -> int:
@@ -115,3 +119,17 @@ def grinqh_prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, c
     sequence (0 * inf is NaN), never another sequence."""
     return _prompt_attention(q, k, v, cu_seqlens_q, cu_seqlens_k,
                              q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale)
+
+
+def grinqh_check_waits() -> None:
+    """Raise if a bounded wait in a kernel of this library on the current device has given up
+    since the last check (the rows concerned are then not valid). Synchronises; not during
+    a capture."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("GRINQH: grinqh_check_waits synchronises and cannot be captured")
+    torch.cuda.synchronize()
+    lost = ctypes.c_uint(0)
+    if cabi().grinqh_take_error_flags(ctypes.byref(lost)) != 0:
+        raise RuntimeError("GRINQH: " + cabi().grinqh_last_error().decode())
+    if lost.value:
+        raise RuntimeError(f"GRINQH: {lost.value} waits in kernels gave up; rows they concern are not valid")

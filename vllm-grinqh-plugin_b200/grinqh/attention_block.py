@@ -18,7 +18,7 @@ from typing import Optional
 
 import torch
 
-from .attention import (grinqh_kv4_append, grinqh_kv4_attention, grinqh_kv4_cache, grinqh_kv4_gather,
+from .attention import (grinqh_check_waits, grinqh_kv4_append, grinqh_kv4_attention, grinqh_kv4_cache, grinqh_kv4_gather,
                         grinqh_prompt_attention)
 from .kernel import grinqh_gemm_or_gemv
 from .utils import pack_codes
@@ -145,6 +145,7 @@ def main(argv: Optional[list] = None) -> None:
         times["prompt_ms"] = 1e3 * _timed(lambda: block.prompt(first))
         times["chunk_ms"] = 1e3 * _timed(lambda: block.prompt(second))
         times["token_ms"] = 1e3 * _timed(lambda: [block.token(x) for x in steps]) / max(1, args.gen)
+    grinqh_check_waits()
     held = block.cache.numel()
     full = 4 * block.tables.numel() * args.page * block.kv * block.dim
     print(json.dumps({"seqs": args.seqs, "prompt": args.prompt, "chunk": args.chunk, "gen": args.gen,
