@@ -88,7 +88,7 @@ const char *grinqh_last_error(void);
  * mbarriers, split-K fix-ups, the fused all-reduce's wait for the other ranks) that
  * gave up since the last call, then reset to 0. Non-zero means a kernel gave up
  * waiting and its output is not valid; once one wait has given up, later waits give
- * up at once until this call clears the count. In grinqh_kv4_attention a wait that gave
+ * up at once until this call clears the count. In the attention calls a wait that gave
  * up (after 2 s, or GRINQH_ATTENTION_WAIT_US microseconds, read on every call) ends with
  * its CTA: the rows it concerns are NaN and no later call is touched. Synchronous.
  * (No reference counterpart: the reference's Triton kernels have no device waits.) */

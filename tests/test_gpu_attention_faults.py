@@ -228,8 +228,8 @@ def test_block_refuses_tokens_behind_its_pages():
 
 # ------------------------------------------------------------------ waits
 def lost_rows(call, want, monkeypatch):
-    """Runs `call` with waits that give up at their first look, `want` being what it returns
-    without: each row is right or NaN, the loss is reported once, and later calls are right."""
+    """Runs `call` with every wait lost, `want` being what it returns without: rows that need
+    nothing are right and all others NaN, the loss is reported once, and later calls are right."""
     monkeypatch.setenv("GRINQH_ATTENTION_WAIT_US", "0")
     outs = [call() for _ in range(3)]
     torch.cuda.synchronize()
@@ -239,13 +239,11 @@ def lost_rows(call, want, monkeypatch):
     with pytest.raises(RuntimeError, match="gave up"):
         G.grinqh_check_waits()
     G.grinqh_check_waits()
-    lost = 0
     for out, lse in outs:
         gone = lse.isnan()
         assert torch.equal(gone, out.isnan().all(-1)) and torch.equal(gone, out.isnan().any(-1))
         assert torch.equal(out[~gone], want[0][~gone]) and torch.equal(lse[~gone], want[1][~gone])
-        lost += int(gone.sum())
-    assert lost > 0
+        assert gone[~want[1].isneginf()].all()
 
 
 @pytest.mark.parametrize("lens,dim,group,new", [([20000, 3, 9000], 128, 64, 1), ([700] * 40, 128, 32, 1), ([50, 0, 31], 64, 32, 4),
@@ -264,3 +262,12 @@ def test_check_of_waits_is_not_captured():
         x += 1
         with pytest.raises(RuntimeError):
             G.grinqh_check_waits()
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv,dim", [([1500], [1500], 2, 1, 128), ([600] * 40, [900] * 40, 8, 2, 64), ([30], [9000], 8, 2, 128),
+                                                ([20, 700, 5], [5000, 700, 0], 4, 2, 64)])
+def test_prompt_attention_waits_are_bounded(nq, nk, heads, kv, dim, monkeypatch):
+    cu = [torch.tensor(np.concatenate([[0], np.cumsum(n)]), dtype=torch.int32).cuda() for n in (nq, nk)]
+    q, k, v = rand((sum(nq), heads, dim), 1), rand((sum(nk), kv, dim), 2), rand((sum(nk), kv, dim), 3)
+    call = lambda: G.grinqh_prompt_attention(q, k, v, *cu)  # noqa: E731
+    lost_rows(call, call(), monkeypatch)

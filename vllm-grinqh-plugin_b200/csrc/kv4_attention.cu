@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
     s_left[warp].flags = 0;
   }
 
-  if (threadIdx.x == 0) s_lost = 0;
+  if (threadIdx.x == 0) s_lost = lost_beforehand(a.wait_ns);
 
   // the next kernel's set-up may overlap this one, as this one's did its predecessor
   allow_dependent_grid();
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
                    v_at = L::kV + t * D + (g ^ (2 * t)) * (4 * W);
     int get = 0;
     uint32_t phase = 0;
-    bool lost = false;  // a wait of this warp was: no record is used from there on
+    bool lost = a.wait_ns == 0;  // a wait of this warp was: no record is used from there on
     while (x < end) {
       const int t0 = seg.at, t1 = min(seg.nt, seg.at + (end - x));  // this piece's records
       if (t0 < t1) {

@@ -26,7 +26,7 @@ inline int allow_smem(const void* kern, std::atomic<uint64_t>& done, size_t byte
 }
 
 // How long a wait within an attention kernel lasts before it is lost: GRINQH_ATTENTION_WAIT_US
-// microseconds (read on every call), by default 2 s.
+// microseconds (read on every call), by default 2 s; with 0 all are lost.
 inline uint64_t attention_wait_ns() {
   const char* e = std::getenv("GRINQH_ATTENTION_WAIT_US");
   return e ? (uint64_t)std::max(0ll, std::min(std::atoll(e), 2000000ll)) * 1000 : kWaitNs;

@@ -32,6 +32,12 @@
 // cut into the same number of parts, items of their own; each writes its sums to the
 // workspace and a second kernel joins them in order.
 //
+// Waits are bounded. Once one of a CTA is lost, nothing more is loaded and no more items are
+// asked for. Those that the CTA has taken over pass through as ever, their products are made
+// with whatever is there, and their rows become NaN; what is in flight is waited for before
+// the CTA ends. (Leaving the loops instead takes a vote at every wait: 475 us -> 553 for a
+// prompt of 16384 tokens.)
+//
 // Measured (bf16, D = 128): a prompt of 16384 tokens, 8 / 2 heads, 475 us, 1.16 PFLOP/s or
 // 69% of a library matrix product's rate; 14 packed prompts of up to 2048 tokens, 32 / 8
 // heads, 110 us, with the tensor pipe active in 46% of the cycles.
@@ -66,6 +72,7 @@ struct PromptArgs {
   int parts;                         // of an item's keys
   int more;                          // whether there are more items than SMs
   float scale_log2;                  // softmax scale * log2(e)
+  uint64_t wait_ns;                  // the longest wait
   float* sums;                       // [item][part][tile]{O[D / 4][row][4], {m, l}[row], token[row]}, for parts > 1
 };
 
@@ -230,9 +237,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   uint64_t* i_full = o_empty + 2;   // [2] an item is known
   uint64_t* i_empty = i_full + 2;   // [2] ... is not needed any more
   uint64_t* c_full = i_empty + 2;   // the answer about a next CTA is there
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_full + 1);
+  uint64_t* done = c_full + 1;      // no product is in flight
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   Item* s_item = reinterpret_cast<Item*>(tmem_slot + 2);  // [2]
   __shared__ __align__(16) uint32_t s_next[4];
+  __shared__ int s_lost;  // a wait of this CTA was lost
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == 9) {
@@ -255,7 +264,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       mbar_init(&i_empty[t], 9);
     }
     mbar_init(c_full, 1);
+    mbar_init(done, 1);
     fence_mbar_init();
+    s_lost = lost_beforehand(a.wait_ns);
   }
   tc_fence_before();
   __syncthreads();
@@ -265,10 +276,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
   wait_prior_grid();
   const uint32_t tmem = *tmem_slot;
   const int tokens = a.tokens;
+  // A wait for data. Who goes on after it was lost is followed by NaN (see the epilogue).
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_or_lose(bar, parity, a.wait_ns, &s_lost); };
+  // Items pass through whatever was lost: whom these wait for goes on in bounded time.
+  auto wait_item = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_drain(bar, parity)); };
   // the k-th item of this CTA, for every warp but the one that finds it
   auto item = [&](int k) {
-    mbar_wait_nocall(&i_full[k & 1], (k >> 1) & 1);
-    const Item it = s_item[k & 1];
+    Item it{0, 0, 0, 0, 0, -1, 0, 0, 0, 0};
+    if (!wait_item(&i_full[k & 1], (k >> 1) & 1)) return it;
+    it = s_item[k & 1];
     __syncwarp();
     if (lane == 0) mbar_arrive(&i_empty[k & 1]);
     return it;
@@ -281,31 +297,33 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
     if (warp == 8) {
       // ---------------------------------------------------------- items, TMA producer
       int stage = 0, round = 1, used = 0;  // ring stage and parity of its release; items so far
+      // Whether memory may be loaded to: it is free, and was not passed on too soon (a load
+      // still on its way would share its barrier with the next).
+      bool lost = false;
+      auto may_load = [&](uint64_t* bar, uint32_t parity) {
+        const bool free = mbar_wait_or_lose(bar, parity, a.wait_ns, &s_lost) &&
+                          *reinterpret_cast<volatile int*>(&s_lost) == 0;
+        lost = lost || !__all_sync(0xffffffffu, free);
+        return !lost;
+      };
       // The next item is asked for when this one's last kAhead loads are left and looked up
       // kFind before its end, so that neither is waited for (a few microseconds an item) and
       // an SM that is behind still takes fewer.
       constexpr int kAhead = 12, kFind = 4;
-      auto ask = [&] {
-        if (lane == 0 && a.more) {
-          fence_proxy_async_smem();  // the last answer has been read
-          mbar_arrive_expect_tx(c_full, 16);
-          next_cta_ask(s_next, c_full);
-        }
-        __syncwarp();
-      };
       const Rows few = a.seqs <= 32 ? sorted_rows(a) : Rows{0, 0, 0, 0};  // the longest start first
       Item it = find_item(a, few, 2 * tokens, (int)blockIdx.x);
       for (int k = 0;; ++k) {
-        if (k >= 2) mbar_wait_nocall(&i_empty[k & 1], ((k >> 1) - 1) & 1);
+        if (k >= 2 && !wait_item(&i_empty[k & 1], ((k >> 1) - 1) & 1)) break;
         if (lane == 0) {
           s_item[k & 1] = it;
           mbar_arrive(&i_full[k & 1]);
         }
         __syncwarp();
         if (it.kv_head < 0) break;
-        const int loads = 2 * max(it.blocks(0, tokens), it.blocks(1, tokens));
+        int loads = 2 * max(it.blocks(0, tokens), it.blocks(1, tokens));
+        if (loads > 0 && used > 0) may_load(q_empty, (used - 1) & 1);
+        if (lost) loads = 0;
         if (loads > 0) {
-          if (used > 0) mbar_wait_nocall(q_empty, (used - 1) & 1);
           ++used;
           if (lane == 0) {
             const uint32_t bytes = a.group * tokens * 128;  // of 64 channels of a tile
@@ -317,15 +335,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
           }
         }
         Item following = it;
+        following.kv_head = -1;
+        bool asked = false;
+        auto ask = [&] {
+          asked = a.more && !lost;
+          if (lane == 0 && asked) {
+            fence_proxy_async_smem();  // the last answer has been read
+            mbar_arrive_expect_tx(c_full, 16);
+            next_cta_ask(s_next, c_full);
+          }
+          __syncwarp();
+        };
         auto find = [&] {
-          const bool answered = a.more && mbar_wait_nocall(c_full, k & 1);
+          const bool answered = asked && wait_item(c_full, k & 1);
           following = find_item(a, few, 2 * tokens, answered ? (int)next_cta_answer(s_next) : -1);
         };
         const int when_ask = max(0, loads - kAhead), when_find = max(0, loads - kFind);
+        bool found = false;
         for (int n = 0; n < loads; ++n) {  // K of block 0, V of block 0, K of block 1, ...
           if (n == when_ask) ask();
-          if (n == when_find) find();
-          mbar_wait_nocall(&empty[stage], round);
+          if (n == when_find) found = true, find();
+          if (!may_load(&empty[stage], round)) break;
           if (lane == 0) {
             mbar_arrive_expect_tx(&full[stage], S::kBytes);
             for (int c = 0; c < S::kAtoms; ++c)
@@ -338,12 +368,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             round ^= 1;
           }
         }
-        if (loads == 0) {
-          ask();
+        if (!found) {
+          if (loads == 0) ask();
           find();
         }
         it = following;
       }
+      // the loads still in flight: of each stage the last, a round back behind `stage`
+      if (used > 0) mbar_drain(q_full, (used - 1) & 1);
+#pragma unroll 1
+      for (int s = 0; s < ST; ++s) mbar_drain(&full[s], s < stage ? round ^ 1 : round);
     } else if (warp == 9) {
       // ---------------------------------------------------------- MMA issuer
       constexpr uint32_t fmt = Act<T>::kBf16 ? 1 : 0;
@@ -355,12 +389,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       const uint64_t k_desc = smem_desc(smem_u32(s_kv), 16, 1024, 2);
       const uint64_t v_desc = smem_desc(smem_u32(s_kv), S::kAtom, 1024, 2);
       int ns = 0, np[2] = {0, 0}, no[2] = {0, 0};  // uses of S, weights and outputs of each tile so far
+      bool free = true;  // no wait for O to be read was lost; once one was, O is not written any more
       auto commit = [&](uint64_t* bar) {
         if (elect_one()) mma_commit(bar);
         __syncwarp();
       };
       auto scores = [&](int t, int at) {  // S = Q_t K^T
-        if (ns > 0) mbar_wait_nocall(s_empty, (ns - 1) & 1);
+        if (ns > 0) wait(s_empty, (ns - 1) & 1);
         ++ns;
         tc_fence_after();
         const uint64_t qd = q_desc + t * (S::kQBytes >> 4), kd = k_desc + at * (S::kBytes >> 4);
@@ -377,9 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         const uint64_t vd = v_desc + at * (S::kBytes >> 4);
         const uint32_t o = tm + S::kO + t * S::kONext, p = tm + S::kP + t * S::kPNext;
         constexpr int kSteps = kKeys / 16, kFirst = S::kFirst;
-        mbar_wait_nocall(kFirst < kSteps ? &p_half[t] : &p_full[t], np[t] & 1);
+        wait(kFirst < kSteps ? &p_half[t] : &p_full[t], np[t] & 1);
         tc_fence_after();
-        if (elect_one()) {
+        if (elect_one() && free) {
           if (steps >= kFirst) {
 #pragma unroll
             for (int kk = 0; kk < kFirst; ++kk)
@@ -392,9 +427,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         }
         __syncwarp();
         if constexpr (kFirst < kSteps) {
-          mbar_wait_nocall(&p_full[t], np[t] & 1);
+          wait(&p_full[t], np[t] & 1);
           tc_fence_after();
-          if (elect_one()) {
+          if (elect_one() && free) {
             if (steps == kSteps) {
 #pragma unroll
               for (int kk = kFirst; kk < kSteps; ++kk) mma_f16_ts(o, p + kk * 8, vd + kk * 128, id_o, 1u);
@@ -409,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       };
       int stage = 0, round = 0, used = 0;  // ring stage of the next block and its parity; items so far
       auto next = [&] {
-        mbar_wait_nocall(&full[stage], round);
+        wait(&full[stage], round);
         const int at = stage;
         if (++stage == ST) {
           stage = 0;
@@ -424,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         const int keys[2] = {uniform(it.keys(0, tokens)), uniform(it.keys(1, tokens))};
         const int nb = max(nbt[0], nbt[1]), begin = uniform(it.begin), m = uniform(it.m);
         if (nb == 0) continue;
-        mbar_wait_nocall(q_full, used & 1);
+        wait(q_full, used & 1);
         ++used;
         const int first = next();
 #pragma unroll
@@ -450,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
             if (j + 1 < nbt[t]) scores(t, ks);  // of the next block, while this one's weights are made
             if (j >= nbt[t]) continue;
             if (j == 0) {
-              if (no[t] > 0) mbar_wait_nocall(&o_empty[t], (no[t] - 1) & 1);
+              if (no[t] > 0) free = wait(&o_empty[t], (no[t] - 1) & 1) && free;
               ++no[t];
             }
             outputs(t, vs, min(kKeys / 16, (keys[t] - (begin + j) * kKeys + 15) / 16), j > 0);
@@ -460,6 +495,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
           commit(&empty[vs]);
         }
       }
+      if (elect_one()) mma_commit(done);
+      __syncwarp();
+      mbar_drain(done, 0);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
@@ -482,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       float m = -INFINITY, ref = 0.f;
       float2 l0 = make_float2(0.f, 0.f), l1 = l0;
       for (int j = 0; j < nb; ++j, ++ns) {
-        mbar_wait_nocall(&s_full[t], ns & 1);
+        wait(&s_full[t], ns & 1);
         tc_fence_after();
         uint32_t sr[kChunks][kCols];
 #pragma unroll
@@ -534,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         for (int c = 0; c < S::kFirst; ++c) weights(c, pk[c]);
         // the weights stay in registers until the block before has been multiplied: P is
         // free then, and O whole
-        if (ns > 0) mbar_wait_nocall(&o_full[t], (ns - 1) & 1);
+        if (ns > 0) wait(&o_full[t], (ns - 1) & 1);
         tc_fence_after();
         if (rescale && j > 0) {
 #pragma unroll 1
@@ -562,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         tc_fence_before();
         mbar_arrive(&p_full[t]);
       }
-      const float l = (l0.x + l0.y) + (l1.x + l1.y);
+      float l = (l0.x + l0.y) + (l1.x + l1.y);
       const bool in = token < it.n && r_token < tokens;
       const int64_t at = (int64_t)(it.q0 + token) * a.heads + it.kv_head * a.group + r_head;
       // The rows of a pair of lanes; their lanes store 64 bytes of one row, then of the other.
@@ -574,8 +612,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
       T* row1 = static_cast<T*>(a.out) + (odd ? at : other) * D + 16 * odd;
       const bool in0 = odd ? other_in : in, in1 = odd ? in : other_in;
       if (nb > 0) {
-        mbar_wait_nocall(&o_full[t], (ns - 1) & 1);
+        wait(&o_full[t], (ns - 1) & 1);
         tc_fence_after();
+        // Whoever passed on what was not there had lost a wait before, and this read follows
+        // what was passed on: the row comes to NaN.
+        if (*reinterpret_cast<volatile int*>(&s_lost)) l = __int_as_float(0x7fffffff);
       }
       const bool none = m == -INFINITY && l == l;  // no score but -inf
       const float inv = 1.0f / l;
@@ -777,6 +818,7 @@ extern "C" int grinqh_prompt_attention(const void* q, const void* k, const void*
   a.group = group;
   a.tokens = kRows / group;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.wait_ns = attention_wait_ns();
   const int64_t items = most_items(total_q, num_seqs, a.tokens, num_kv_heads);
   a.parts = parts_for(items, total_k, num_seqs, sm_count());
   a.more = items * a.parts > sm_count();

@@ -47,6 +47,16 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t by
 #ifndef GRINQH_WAIT_HINT_NS
 #define GRINQH_WAIT_HINT_NS 1000000u
 #endif
+template <uint32_t kHintNs>
+__device__ __forceinline__ bool mbar_try_wait_for(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(kHintNs)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
 #if GRINQH_WAIT_HINT_NS == 0
@@ -106,23 +116,32 @@ static __device__ __noinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   }
 }
 
-// A wait that a CTA can lose: true when the phase completes; false after `limit` ns (with 0
-// one look is taken), or when another wait of the CTA has been lost (`lost`, in shared
-// memory, set and counted by the first). What it waited for may then not be used: the caller
-// makes its outputs NaN and waits for its own copies (mbar_drain). Inline as a whole, since
-// a kernel that splits its registers between warps (setmaxnreg) can call no function.
+// A wait that a CTA can lose: true when the phase completes; false after `limit` ns, or when
+// another wait of the CTA has been lost (`lost`, in shared memory, set and counted by the
+// first). What it waited for is then not there: the caller makes its outputs NaN and waits
+// for its own copies (mbar_drain) before it ends. Inline as a whole, since a kernel that
+// splits its registers between warps (setmaxnreg) can call no function.
+constexpr uint32_t kLoseHintNs = 20000;  // a try: what is left of a kernel that has lost one ends soon
 __device__ __forceinline__ bool mbar_wait_or_lose(uint64_t* bar, uint32_t parity, uint64_t limit, int* lost) {
-  if (limit == 0 ? mbar_test(bar, parity) : mbar_try_wait(bar, parity)) return true;
+  if (mbar_try_wait_for<kLoseHintNs>(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
 #pragma unroll 1
   while (*reinterpret_cast<volatile int*>(lost) == 0) {
     if (globaltimer_ns() - t0 >= limit) {
       if (atomicExch(lost, 1) == 0) atomicAdd(&g_wait_timeouts, 1u);
+      __threadfence_block();  // who sees what follows sees this
       return false;
     }
-    if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait_for<kLoseHintNs>(bar, parity)) return true;
   }
   return false;
+}
+
+// What `lost` begins with: with a limit of 0 all waits are lost beforehand (one thread calls).
+__device__ __forceinline__ int lost_beforehand(uint64_t limit) {
+  if (limit != 0) return 0;
+  atomicAdd(&g_wait_timeouts, 1u);
+  return 1;
 }
 
 // Waits for copies or products that still write this CTA's memory, whatever was lost.
@@ -134,24 +153,6 @@ __device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
   atomicAdd(&g_wait_timeouts, 1u);
   return false;
-}
-
-// mbar_wait inline as a whole: a kernel that splits its registers between warps
-// (setmaxnreg) can call no function.
-__device__ __forceinline__ bool mbar_wait_nocall(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-#pragma unroll 1
-  for (uint32_t it = 1;; ++it) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 255u) == 0) {
-      if (*reinterpret_cast<volatile unsigned*>(&g_wait_timeouts) != 0u) return false;
-      if (globaltimer_ns() - t0 > kWaitNs) {
-        atomicAdd(&g_wait_timeouts, 1u);
-        return false;
-      }
-    }
-  }
 }
 
 // mbar_wait with its first try inline: no call on the common path, where the phase

@@ -6,8 +6,8 @@ decoder layer and want the cache as small as GRINQH's weights. A cache is a uint
 [pages, kv heads, page_size / 16, record] (``grinqh_kv4_cache``); its layout is in
 ``include/grinqh_b200.h``. Every function raises on CPU tensors, runs on the current
 stream without synchronising, and can be recorded into a CUDA graph. Waits inside the
-kernels are bounded (2 s, or ``GRINQH_ATTENTION_WAIT_US``); rows of ``kv4_attention`` whose wait was lost
-come out as NaN, and ``grinqh_check_waits`` raises.
+kernels are bounded (2 s, or ``GRINQH_ATTENTION_WAIT_US``); rows whose wait was lost come
+out as NaN, and ``grinqh_check_waits`` raises.
 """
 from __future__ import annotations
 
