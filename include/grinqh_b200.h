@@ -314,6 +314,10 @@ int grinqh_kv4_gather(const uint8_t *cache, int dtype, int64_t num_pages, int pa
  * a page outside the cache are left out. out [num_seqs, new_tokens, num_heads, D] dtype
  * and lse [num_seqs, new_tokens, num_heads] fp32 are contiguous. num_heads is a multiple
  * of num_kv_heads, new_tokens * num_heads / num_kv_heads at most 32.
+ * A weight is held to 2^-11 of itself and to 2^-35 of its row's largest, times the largest
+ * of V's scales of the sequence and head over the scale it belongs to: groups and tokens
+ * with scales below 2^-24 of the largest lose what sets their values apart. Sums of weights
+ * times values are made in fp32 before the division.
  * flags: GRINQH_WORKSPACE_ZEROED as for the linears. */
 size_t grinqh_kv4_attention_workspace_size(int64_t num_seqs, int new_tokens, int num_heads, int num_kv_heads,
                                            int head_dim);

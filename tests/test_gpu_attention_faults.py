@@ -1,7 +1,8 @@
 """What a reading of the attention operators and of what they share with the linears found
 wrong, each held by a test: workspaces of captured graphs,
 caches without heads, expanded inputs, joins of many sequences in a CTA, a block
-that is full, waits that are lost.
+that is full, waits that are lost, values of V
+of very different size.
 """
 import numpy as np
 import pytest
@@ -11,6 +12,8 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():
     pytest.skip("needs a CUDA device", allow_module_level=True)
+
+from oracle import attention as A  # noqa: E402
 
 from grinqh import attention as G  # noqa: E402
 from grinqh.kernel import grinqh_gemm_or_gemv  # noqa: E402
@@ -271,3 +274,63 @@ def test_prompt_attention_waits_are_bounded(nq, nk, heads, kv, dim, monkeypatch)
     q, k, v = rand((sum(nq), heads, dim), 1), rand((sum(nk), kv, dim), 2), rand((sum(nk), kv, dim), 3)
     call = lambda: G.grinqh_prompt_attention(q, k, v, *cu)  # noqa: E731
     lost_rows(call, call(), monkeypatch)
+
+
+# ------------------------------------------------------------------ range
+def one_sequence(k, v, group, page=16):
+    """A cache of k and v [n, 1, D], tables and lengths, and what it holds in 64 bits."""
+    n = k.shape[0]
+    pages = -(-n // page)
+    cache = G.grinqh_kv4_cache(pages, 1, k.shape[2], page, group)
+    G.grinqh_kv4_append(k, v, cache, torch.arange(n).cuda(), group)
+    held = A.read_tokens(cache.cpu().numpy().reshape(-1, cache.shape[3]), k.shape[2], group, "bf16")
+    tables = torch.arange(pages, dtype=torch.int32).cuda()[None]
+    return cache, tables, torch.tensor([n], dtype=torch.int32).cuda(), [x[:n, None] for x in held]
+
+
+def scales_of(v, group):
+    g = v.reshape(*v.shape[:-1], -1, group)
+    return ((g.max(-1, keepdims=True) - g.min(-1, keepdims=True)) / 15 * np.ones(group)).reshape(v.shape)
+
+
+@pytest.mark.parametrize("what", ["group", "token"])
+@pytest.mark.parametrize("power", [12, 20, 24])
+@pytest.mark.parametrize("dim,group,heads", [(128, 64, 4), (64, 32, 12), (128, 32, 1)])
+def test_cached_attention_of_values_of_very_different_size(what, power, dim, group, heads):
+    """One group of V, or one token that hardly counts, is 2^power larger than the rest. A weight
+    is off by 2^-11 of itself (twice: its own rounding and the scale's product) and, in f16's smallest
+    step, by 2^-35 of the row's largest times the largest scale over its own; a code is at most 15."""
+    n = 300
+    k, v, q = rand((n, 1, dim), 1), rand((n, 1, dim), 2), rand((1, heads, dim), 3)
+    big = 2.0**power
+    if what == "group":
+        v[:, :, :group] *= big
+    else:
+        q = q.abs()
+        k[7], v[7] = -3.0, v[7] * big
+    cache, tables, lens, (kr, vr) = one_sequence(k, v, group)
+    out, lse = G.grinqh_kv4_attention(q, cache, tables, lens, group)
+    x = q.double().cpu().numpy()
+    ref, ref_lse, _, reach = A.attention(x, kr, vr, dim**-0.5)
+    s = scales_of(vr, group)
+    size = A.attention(x, kr, np.abs(vr) + 15 * s, dim**-0.5)[2]
+    top = (x[0] @ kr[:, 0].T).max(-1) * dim**-0.5
+    share = np.exp(top - ref_lse[0])[None, :, None]  # of the row's largest weight
+    d = 2.0**-20 * (3 * reach.max() + 1)
+    off = np.abs(out.double().cpu().numpy() - ref)
+    limit = (2.0**-10 + 2 * d) * size + 2.0**-8 * np.abs(ref) + n * share * 15 * 2.0**-35 * s.max() + 2.0**-20 * size
+    assert (off <= limit).all(), f"worst {np.max(off / limit)} of the bound"
+
+
+@pytest.mark.parametrize("q_power,k_power,v_power", [(0, 0, 118), (0, 0, -110), (117, -119, 0), (-100, 100, 0)])
+def test_cached_attention_of_huge_and_tiny_values(q_power, k_power, v_power):
+    """Values near the ends of bf16's range, with scores and outputs within it."""
+    n = 100
+    k, v, q = rand((n, 1, 128), 1) * 2.0**k_power, rand((n, 1, 128), 2).clamp(-3, 3), rand((1, 4, 128), 3) * 2.0**q_power
+    cache, tables, lens, (kr, vr) = one_sequence(k, v * 2.0**v_power, 128)
+    out, lse = G.grinqh_kv4_attention(q, cache, tables, lens, 128)
+    ref, ref_lse, _, _ = A.attention(q.double().cpu().numpy(), kr, vr, 128**-0.5)
+    # weights in 11 bits times codes up to 3 |v|, out rounded to 8; a score's products near 2^-126 lose bits: 1 %
+    size = np.abs(vr).max()
+    assert np.abs(out.double().cpu().numpy() - ref).max() <= 0.01 * size
+    assert np.abs(lse.double().cpu().numpy() - ref_lse).max() <= 0.01 * (1 + np.abs(ref_lse).max())

@@ -46,8 +46,8 @@ namespace grinqh {
 namespace {
 
 constexpr int kMaxRows = 32;  // new tokens x query heads of a kv head
-constexpr float kSlack = 1024.0f;  // a lane's weights of a step may sum to this before the maximum follows
-constexpr int kTopScale = 4;       // V scales x vf stay below 2^(kTopScale + 1): weights x that within f16's range
+constexpr float kSlack = 16.0f;  // a lane's weights of a step may sum to this before the maximum follows
+constexpr int kTopScale = 10;    // V scales x vf stay below 2^(kTopScale + 1): weights x that within f16's range
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr uint32_t kFull = 0xffffffffu;
 
@@ -468,7 +468,8 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
           float top = fmaxf(Act<T>::to_f(most.x), Act<T>::to_f(most.y));
           top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
           top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
-          const float up = top > 0.f ? power_for(top, 13) : 1.0f;
+          // (above 2^-103, for down; only rows of 2^116 and more come closer to f16's end)
+          const float up = top > 0.f ? fmaxf(power_for(top, 13), 0x1p-103f) : 1.0f;
           float sum[NG];
 #pragma unroll
           for (int i = 0; i < NG; ++i) sum[i] = 0.f;
@@ -506,7 +507,11 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
 
         float m[NT][2], ref[NT][2], l[NT][2], z[NT][2][NG];
         float o[2 * W][NT][4];
-        // weights enter the product as p scale vf; back = 1 / vf, scales stay below the limit
+        // Weights enter the product as p scale vf; back = 1 / vf, scales stay below the limit.
+        // vf follows the largest scale of the piece, so f16's smallest step is 2^-35 of that
+        // one's weight 1: a scale 2^20 times smaller has its weights to 2^-16 of the largest. With
+        // kSlack 1024 these were 2^-29 and 2^-10, for the same times; with 4, which would
+        // leave 2^-37, the maximum follows too often (33 sequences with drafts, 31.4 us -> 32.5).
         float vf = 0x1p100f, back = 0x1p-100f, limit = (float)(2 << kTopScale) * back;
         bool first = true;
 #pragma unroll
@@ -762,11 +767,11 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
             for (int w = 0; w < W; ++w) {
               const int gi = w / L::kGroupWords, j = w % L::kGroupWords;
               const int d = gi * GS + g * (GS / 8) + 4 * j;
-              const float f = back * 16777216.0f;
-              const float4 v = make_float4(fmaf(o[2 * w][n][c], f, z[n][c][gi]),
-                                           fmaf(o[2 * w][n][2 + c], f * 0.0625f, z[n][c][gi]),
-                                           fmaf(o[2 * w + 1][n][c], f, z[n][c][gi]),
-                                           fmaf(o[2 * w + 1][n][2 + c], f * 0.0625f, z[n][c][gi]));
+              // in two steps: back x 2^24 may be more than fp32 holds
+              const float4 v = make_float4(fmaf(o[2 * w][n][c] * back, 0x1p24f, z[n][c][gi]),
+                                           fmaf(o[2 * w][n][2 + c] * back, 0x1p20f, z[n][c][gi]),
+                                           fmaf(o[2 * w + 1][n][c] * back, 0x1p24f, z[n][c][gi]),
+                                           fmaf(o[2 * w + 1][n][2 + c] * back, 0x1p20f, z[n][c][gi]));
               if (began || goes) {
                 *reinterpret_cast<float4*>(sums + r * P::kRow + d) = v;
               } else if (r < rows) {

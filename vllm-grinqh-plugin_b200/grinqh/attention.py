@@ -99,7 +99,8 @@ def grinqh_kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_tables: tor
     counts the new tokens, which have been appended; ``block_tables`` (int32, [seqs,
     width]) lists each sequence's pages. Query j of a sequence of length n sees tokens
     0 .. n - new + j; one that sees none gives zeros and lse = -inf. ``lse`` is the
-    natural logarithm of the sum of exp(softmax_scale * q . k)."""
+    natural logarithm of the sum of exp(softmax_scale * q . k). Groups of V whose scale is
+    less than 2^-24 of the largest of the sequence and head are summed less exactly."""
     return _kv4_attention(q, cache, block_tables, seq_lens, group_size,
                           q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale)
 
