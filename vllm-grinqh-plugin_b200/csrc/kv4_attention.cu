@@ -32,8 +32,10 @@
 //
 // Measured (bf16, D = 128, group 128, 32 / 8 heads): 5 sequences of 50001 to 131072 tokens,
 // 111 us, 67% of the copy bandwidth (the loop runs at 90%; the rest is the ends, and the SMs
-// whose loads take longer); 64 of 512 to 768, group 64, 26 us, 28%; one of 301, 8 us, one
-// after another: looking up pages, a record, joining.
+// whose loads take longer); 64 of 8192, 121 us, 72%; 64 of 512 to 768, group 64, 26 us, 28%;
+// one of 301, 8 us, one after another: looking up pages, a record, joining. 33 of up to 9000
+// with 4 new tokens (fp16, D = 64, group 32, 24 / 8 heads), 31.4 us: 12 query rows a record, in
+// a kernel that spills (Plan), at 46% of the issue slots, and the same joins.
 #include "kv4.cuh"
 #include "kv4_attention.cuh"
 #include "launch.cuh"
@@ -76,7 +78,10 @@ template <int D, int GS, int NT>
 struct Plan {
   static constexpr int kRows = 8 * NT;
   // Warps that compute, beside the one that loads: one CTA per SM, and 128 registers a
-  // thread, or 255 where the sums of 16 rows x 128 channels take 128 of them.
+  // thread, or 255 where the sums of 16 rows x 128 channels take 128 of them. 15 rings of
+  // D = 128, group 32 would not fit the shared memory, 14 do. Not all instances fit their
+  // registers. Bytes of a thread's spilled stores: 16 rows, D = 64, 280 to 300 (group 32) and 100
+  // (group 64); 8 rows, D = 128, 200 to 225 (group 32) and 20 to 30; the others up to 44.
   static constexpr int kWarps = NT == 2 && D == 128 ? 7 : (D == 128 && GS == 32 ? 14 : 15);
   static constexpr int kThreads = 32 * (kWarps + 1);
   // Stages of two records.
@@ -91,7 +96,8 @@ struct Plan {
 };
 
 // What a sequence and head costs beside its records, in records: q, finishing or joining.
-// 33 sequences of up to 9000 tokens, 8 kv heads: 55.2 us with 4, 52.5 with 8, 53.9 with 16.
+// 33 sequences of up to 9000 tokens with 4 new ones, 8 kv heads: 38.2 us with 4, 31.4 with 8,
+// 33.8 with 16; 64 of 512 to 768, 27.2, 26.0 and 26.5; long ones, 110.9, 111.2 and 111.8.
 constexpr int kCost = 8;
 
 __device__ __forceinline__ int tiles_of(const Kv4AttnArgs& a, int b) {
@@ -696,7 +702,7 @@ __global__ void __launch_bounds__(Plan<D, GS, NT>::kThreads, 1) kv4_attention_ke
                   // What the 11 bits lose is given back for a code of 7.5, the middle of the
                   // range, so that the error left is that of v's spread and not of its offset:
                   // fp16 outputs would show it (3.5e-4 relative without, 2.4e-4 with), bf16's
-                  // own rounding (1.7e-3) hides it.
+                  // own rounding (1.7e-3, with fp32 weights too) hides it, so bf16 goes without.
                   const float2 ra = __half22float2(*reinterpret_cast<const __half2*>(&ha));
                   const float2 rb = __half22float2(*reinterpret_cast<const __half2*>(&hb));
                   z[n][0][k] = fmaf((u[0] - ra.x) + (u[2] - rb.x), 7.5f * back, z[n][0][k]);

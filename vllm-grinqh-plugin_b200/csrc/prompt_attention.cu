@@ -25,8 +25,14 @@
 // products follow one another as S0 O0 S1 O1, each with a whole round of the others to
 // wait in. A 128 x 128 x 16 product takes 102 cycles with both operands in shared memory
 // and 78 with A in TMEM (measured alone; 64 would be full rate), 2880 a round at head_dim
-// 128: that is what bounds the kernel there, and the exponentials, 8 cycles for a warp's
-// 32 of them or 2048 a round, at head_dim 64.
+// 128; the exponentials, 8 cycles for a warp's 32 of them, 2048 a round.
+//
+// What bounds it, by the SMs' active cycles: a prompt of 16384 tokens at head_dim 128 takes 3080
+// cycles a round, so the products 94% of them, and 5% more until the last SM ends. 14 packed
+// prompts of up to 2048 tokens take 4270 a round: with 6 items an SM, half masked blocks,
+// starts and epilogues count, in which one of the two pipes waits. 7 chunks after prefixes at
+// head_dim 64, 3280 a round, have 1.6 items an SM that are not cut: SMs are active for 72 to 124
+// thousand cycles, 94 on average, of which exponentials are 59%.
 //
 // Where there are few items for the SMs (a chunk after a long prefix), each item's keys are
 // cut into the same number of parts, items of their own; each writes its sums to the
@@ -39,8 +45,8 @@
 // prompt of 16384 tokens.)
 //
 // Measured (bf16, D = 128): a prompt of 16384 tokens, 8 / 2 heads, 475 us, 1.16 PFLOP/s or
-// 69% of a library matrix product's rate; 14 packed prompts of up to 2048 tokens, 32 / 8
-// heads, 110 us, with the tensor pipe active in 46% of the cycles.
+// 69% of a library matrix product's rate (the SMs at 1.65 GHz), with the tensor pipe active in
+// 66% of the cycles; 14 packed prompts of up to 2048 tokens, 32 / 8 heads, 111 us and 46%.
 //
 // Keys past the sequence's end belong to another sequence and may hold anything: their
 // scores are masked, the O += P V steps of 16 keys past the last visible one are not
@@ -554,6 +560,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_attention_kernel(const __g
         const bool rescale = __any_sync(0xffffffffu, up);
         if (rescale) l0.x *= f, l0.y *= f, l1.x *= f, l1.y *= f;
         const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
+        // Weights are rounded to the type of V, since a product's operands have one: each by
+        // up to 2^-9 (bf16) or 2^-12 of itself, either way, and l sums them before. Outputs are off
+        // by 1.9e-3 (bf16) and 2.9e-4 (fp16) in the 2-norm, against 1.6e-3 and 2.1e-4 with fp32
+        // weights, where only their own rounding is left; V and P in fp32 would take twice the
+        // products. The exponential's own error is 2^-22.
         auto weights = [&](int c, uint32_t (&pk)[kCols / 2]) {
 #pragma unroll
           for (int i = 0; i < kCols / 2; ++i) {
