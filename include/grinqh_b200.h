@@ -289,7 +289,9 @@ int64_t grinqh_kv4_record_bytes(int head_dim, int group_size);
 /* Quantize k, v [tokens, num_kv_heads, D] (strides in elements, D contiguous) into the
  * cache; token i goes to place slots[i] = page * page_size + offset. Per token, head and
  * group: zero = min x, scale = dtype((max - min) / 15), code = clamp(rint((x - zero) *
- * (1 / scale)), 0, 15) in fp32 (0 for a scale below 2^-126). A slot outside the cache (-1 for
+ * (1 / scale)), 0, 15) in fp32 (0 for a scale below 2^-126). A group with a value that is not
+ * finite, or whose max - min is not in fp32, reads back as NaN; values that the scale's
+ * rounding takes past the largest of dtype read back infinite. A slot outside the cache (-1 for
  * padding) writes nothing; slots of one call must differ. k, v and their strides are
  * 16-byte aligned. */
 int grinqh_kv4_append(const void *k, const void *v, int dtype, int64_t tokens, int num_kv_heads, int head_dim,
